@@ -225,6 +225,121 @@ int jx_matmul_qkv_quant_f32_dev(jx_qmatrix* Wq, jx_qmatrix* Wk, jx_qmatrix* Wv, 
  * device: x [k] fp32 -> k/32 blocks of 34 bytes (fp16 d + 32 int8).  Host pointers. */
 int jx_quantize_row_q8_0(const float* x, void* blocks, int64_t k);
 
+/* ---- paged 8-bit key/value cache and the attention over it ---------------- */
+
+/* The step between the q / k / v projection and the output projection of a layer.  The reference keeps its cache in
+ * fp16, one region per slot (src/transformer.cpp:2029-2046, 2448-2582); here it is the caller's device memory in pages,
+ * int8 with one fp32 scale for each block of JX_KV_BLOCK tokens and head, shared between sequences by reference counts.
+ *
+ *   codes  int8 [n_layers][n_pages][K, V][n_kv_heads][page_tokens / 32][32 * head_dim], 16-byte aligned
+ *            K block: [head_dim / 16][32 tokens][16]: byte (c, t, i) is dimension 16 c + i of token t
+ *            V block: [2][head_dim][16]: byte (h, d, 8 (a & 1) + 4 (a >> 1) + b) is dimension d of token 8 a + 4 h + b (a, b < 4)
+ *   scales fp32 [n_layers][n_pages][K, V][n_kv_heads][page_tokens / 32]: a value is code * scale
+ *   table  int32 [max_seqs][max_pages]: the pages of each slot (a slot holds one sequence or none)
+ *   len    int32 [max_seqs]: its tokens (0: none).  Entries of the table behind the last page mean nothing.
+ *   ref    int32 [n_pages]: how many slots hold a page (0: free)
+ *   status int32 [JX_KV_STATUS_WORDS]: word 0 the JX_KV_* bits below, word 1 the pages in use after jx_kv_compact
+ *   scratch int32 [jx_kv_scratch_words()]: workspace of the page operations
+ * The first JX_KV_* bit that a call of jx_kv_append sets may leave its other sequences' tokens written.
+ * A program zeroes len, ref and status once; codes, scales, table and scratch need no initial values.
+ *
+ * Errors that only the device can see set a bit of the status word.  While it is not zero, jx_kv_append and the page
+ * operations do nothing and jx_kv_attention writes NaN: read it (4 bytes) where results are read, zero it to go on.
+ * A page operation that reports changed nothing.
+ *
+ * Every call is enqueued on `stream` (NULL = default stream), returns without synchronizing, allocates nothing, reads
+ * lengths, tables and lists on the device only and may be captured in a graph.  Calls that change a cache must be
+ * ordered with every other call on it; jx_kv_attention calls may overlap each other, each with a workspace of its own. */
+#define JX_KV_BLOCK 32
+#define JX_KV_STATUS_WORDS 4
+enum {
+    JX_KV_BAD_PAGE = 1,  /* a table entry names no page of the cache                                      */
+    JX_KV_BAD_ARG = 2,   /* a slot, length or row range out of its limits, or a slot twice in one list    */
+    JX_KV_NO_PAGES = 4,  /* the call needs more free pages than there are                                 */
+    JX_KV_SHARED = 8     /* jx_kv_append into a page that another slot holds too: that page is left alone  */
+};
+
+typedef struct jx_kv_cache {
+    int32_t device;       /* of the memory below; jx_moe_init has been called for it */
+    int32_t n_layers;
+    int32_t n_pages;
+    int32_t page_tokens;  /* 32, 64, 128 or 256 */
+    int32_t n_kv_heads;
+    int32_t head_dim;     /* a multiple of 32 up to 256 */
+    int32_t max_seqs;
+    int32_t max_pages;    /* pages of the longest sequence */
+    int8_t* codes;
+    float* scales;
+    int32_t* table;
+    int32_t* len;
+    int32_t* ref;
+    int32_t* status;
+    int32_t* scratch;
+} jx_kv_cache;
+
+/* int32 words of `scratch`, 0 for a cache that the calls would refuse */
+int64_t jx_kv_scratch_words(const jx_kv_cache* cache);
+
+/* The rows of one call: for sequence i < n_seqs the rows row_start[i] .. row_start[i + 1] - 1, which are the LAST tokens
+ * of slot seqs[i], in order (its length counts them already).  No slot comes twice in one append. */
+typedef struct jx_kv_batch {
+    int32_t n_seqs;
+    int32_t n_rows;            /* rows of the arrays; rows that belong to no sequence are left alone  */
+    int32_t max_rows;          /* no sequence has more rows (a sequence with more: JX_KV_BAD_ARG)      */
+    int32_t max_len;           /* about the longest sequence: how the work is divided, not a limit; 0: unknown */
+    const int32_t* seqs;       /* device int32 [n_seqs] or NULL (slot i)                               */
+    const int32_t* row_start;  /* device int32 [n_seqs + 1] or NULL (one row each, n_rows == n_seqs)   */
+} jx_kv_batch;
+
+/* Page operations over lists of n distinct slots (device int32 [n]).
+ *   reserve: room for n_new[i] tokens (NULL: one each) behind slots[i], and its length grows by them: first reserve,
+ *            then append in every layer.  Pages are taken lowest free first, in the order of the list.
+ *   trim:    slots[i] keeps its first new_len[i] tokens at most (NULL: none, the slot is freed).  A last page that is
+ *            partly used and shared is copied, so that it can be written again.
+ *   fork:    dst[i] becomes src[i] as it was before the call: full pages are shared, a partly used last page is copied to
+ *            a page that was free before the call.  What dst[i] held is freed.  A source may come several times and may
+ *            be a destination too (dst[i] == src[i] changes nothing).
+ *   compact: the pages in use become 0 .. count - 1: each one behind them moves, in order, to the next free place.
+ * Pages are copied in every layer. */
+int jx_kv_reserve(const jx_kv_cache* cache, const int32_t* slots, const int32_t* n_new, int32_t n, void* stream);
+int jx_kv_trim(const jx_kv_cache* cache, const int32_t* slots, const int32_t* new_len, int32_t n, void* stream);
+int jx_kv_fork(const jx_kv_cache* cache, const int32_t* src, const int32_t* dst, int32_t n, void* stream);
+int jx_kv_compact(const jx_kv_cache* cache, void* stream);
+
+/* Keys and values of the batch's rows into `layer`.  k, v: [n_rows][n_kv_heads][head_dim] of `type` (JX_TYPE_F32, F16 or
+ * BF16) with row_stride elements between rows (0: n_kv_heads * head_dim); any alignment of the type.
+ * The scale of a block is max(amax / 127 of its new tokens, its scale so far if it holds earlier tokens), 0 below 2^-120;
+ * a code is the nearest integer to value / scale.  Where the scale grows, the block's earlier codes are rounded again
+ * to it.  A value that is not finite makes the scale of its block NaN: the whole block reads as NaN. */
+int jx_kv_append(const jx_kv_cache* cache, const jx_kv_batch* batch, int32_t layer, int32_t type, const void* k, const void* v,
+                 int64_t row_stride, void* stream);
+
+/* Attention of the batch's rows over their sequences in `layer`.  Row at position p (its place in the sequence), head j,
+ * over the visible tokens t of kv head j / (n_heads / n_kv_heads):
+ *   x_t = scale * (q . K_t);  softcap > 0: x_t = softcap * tanh(x_t / softcap);  alibi: x_t += alibi[j] * (t - p)
+ *   out = sum_t exp(x_t) V_t / sum_t exp(x_t), zeros where nothing is visible
+ * visible: causal: t <= p, otherwise every token of the sequence; window > 0: also t > p - window.
+ * q, out: [n_rows][n_heads][head_dim] of `type` with q_stride / out_stride elements between rows (0: n_heads * head_dim),
+ * any alignment of the type; out may be q.  type F32 keeps 21 bits of q against its row's largest value and the
+ * weights in 22 bits; F16 and BF16 keep 14 and 11.  A row of q with a value that is not finite gives NaN; one whose
+ * values are all below 2^-100 counts as zeros.
+ * ws: device memory of jx_kv_attention_workspace() bytes (0: may be NULL), 16-byte aligned, for this call alone. */
+typedef struct jx_attention {
+    int32_t n_heads;     /* a multiple of the cache's n_kv_heads */
+    int32_t type;        /* of q and out */
+    float scale;         /* head_dim^-0.5 usually */
+    float softcap;       /* 0: none */
+    int32_t window;      /* 0: none */
+    int32_t causal;      /* 0 or 1 */
+    int64_t q_stride;
+    int64_t out_stride;
+    const float* alibi;  /* device fp32 [n_heads] or NULL */
+} jx_attention;
+
+size_t jx_kv_attention_workspace(const jx_kv_cache* cache, const jx_kv_batch* batch, const jx_attention* attention);
+int jx_kv_attention(const jx_kv_cache* cache, const jx_kv_batch* batch, const jx_attention* attention, int32_t layer,
+                    const void* q, void* out, void* ws, size_t ws_bytes, void* stream);
+
 /* ---- GGUF model files (host only) ---------------------------------------- */
 
 /* A GGUF v2/v3 file mapped read-only and parsed: header, metadata, tensor table

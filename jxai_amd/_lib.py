@@ -21,6 +21,13 @@ JX_FWD_RESIDUAL = 1 << 4
 JX_FWD_UNFUSED = 1 << 5
 JX_FWD_TEST_GIVEUP = 1 << 6  # test hook: the fused one-token step's waits give up (outputs invalid)
 
+JX_KV_BLOCK = 32
+JX_KV_STATUS_WORDS = 4
+JX_KV_BAD_PAGE = 1
+JX_KV_BAD_ARG = 2
+JX_KV_NO_PAGES = 4
+JX_KV_SHARED = 8
+
 JX_ACT_SILU = 0
 JX_ACT_GELU_TANH = 1
 
@@ -35,6 +42,8 @@ EXPORTS = [
     "jx_gguf_get_u32", "jx_gguf_get_f32", "jx_gguf_get_str", "jx_gguf_moe_layer_desc", "jx_gguf_last_error",
     "jx_matmul_quant_f32_dev", "jx_matmul_qkv_quant_f32_dev", "jx_moe_layer_status",
     "jx_build_id",
+    "jx_kv_scratch_words", "jx_kv_reserve", "jx_kv_trim", "jx_kv_fork", "jx_kv_compact", "jx_kv_append",
+    "jx_kv_attention_workspace", "jx_kv_attention",
 ]
 
 _fp = C.POINTER(C.c_float)
@@ -55,6 +64,26 @@ class LayerDesc(C.Structure):
         ("activation", C.c_int32), ("router_type", C.c_int32),
         ("ffn_norm", _vp), ("post_ffw_norm", _vp), ("rms_norm_eps", C.c_float),
     ]
+
+
+class KVCacheDesc(C.Structure):
+    """jx_kv_cache."""
+    _fields_ = [(name, C.c_int32) for name in ("device", "n_layers", "n_pages", "page_tokens", "n_kv_heads", "head_dim",
+                                               "max_seqs", "max_pages")]
+    _fields_ += [(name, _vp) for name in ("codes", "scales", "table", "len", "ref", "status", "scratch")]
+
+
+class KVBatchDesc(C.Structure):
+    """jx_kv_batch."""
+    _fields_ = [("n_seqs", C.c_int32), ("n_rows", C.c_int32), ("max_rows", C.c_int32), ("max_len", C.c_int32),
+                ("seqs", _vp), ("row_start", _vp)]
+
+
+class AttentionDesc(C.Structure):
+    """jx_attention."""
+    _fields_ = [("n_heads", C.c_int32), ("type", C.c_int32), ("scale", C.c_float), ("softcap", C.c_float),
+                ("window", C.c_int32), ("causal", C.c_int32), ("q_stride", C.c_int64), ("out_stride", C.c_int64),
+                ("alibi", _vp)]
 
 
 class JxError(RuntimeError):
@@ -119,6 +148,17 @@ def lib() -> C.CDLL:
     L.jx_gguf_get_str.argtypes = [_vp, C.c_char_p, C.POINTER(C.c_char_p)]
     L.jx_gguf_moe_layer_desc.argtypes = [_vp, C.c_int32, C.POINTER(LayerDesc)]
     L.jx_gguf_last_error.restype = C.c_char_p
+    cache, batch = C.POINTER(KVCacheDesc), C.POINTER(KVBatchDesc)
+    L.jx_kv_scratch_words.argtypes = [cache]
+    L.jx_kv_scratch_words.restype = C.c_int64
+    L.jx_kv_reserve.argtypes = [cache, _vp, _vp, C.c_int32, _vp]
+    L.jx_kv_trim.argtypes = [cache, _vp, _vp, C.c_int32, _vp]
+    L.jx_kv_fork.argtypes = [cache, _vp, _vp, C.c_int32, _vp]
+    L.jx_kv_compact.argtypes = [cache, _vp]
+    L.jx_kv_append.argtypes = [cache, batch, C.c_int32, C.c_int32, _vp, _vp, C.c_int64, _vp]
+    L.jx_kv_attention_workspace.argtypes = [cache, batch, C.POINTER(AttentionDesc)]
+    L.jx_kv_attention_workspace.restype = C.c_size_t
+    L.jx_kv_attention.argtypes = [cache, batch, C.POINTER(AttentionDesc), C.c_int32, _vp, _vp, _vp, C.c_size_t, _vp]
     _lib = L
     return L
 

@@ -18,6 +18,7 @@
 #include "../../include/jxmoe.h"
 #include "jxmoe_device.h"
 #include "jxmoe_kernels.h"
+#include "jxmoe_kv.h"
 
 namespace {
 
@@ -1044,6 +1045,19 @@ struct Scratch {
 };
 
 }  // namespace
+
+namespace jx {
+
+int api_fail(int code, const std::string& msg) { return fail(code, msg); }
+
+int api_device(int device) {
+    if (device < 0 || device >= MAX_DEVICES || !g_scratch[device].load())
+        return fail(JX_ERR_NODEVICE, "jx_moe_init has not been called for the cache's device");
+    HIPCHK(hipSetDevice(device));
+    return JX_OK;
+}
+
+}  // namespace jx
 
 extern "C" {
 
