@@ -40,6 +40,22 @@ __device__ __forceinline__ void store1(void* p, int type, int64_t i, float v) {
         reinterpret_cast<uint16_t*>(p)[i] = (uint16_t)(type == JX_TYPE_F16 ? half_bits(v) : bf16_bits(v));
 }
 
+// Four consecutive values; vec: their place is aligned to four values
+__device__ __forceinline__ void store4(void* p, int type, int64_t i, bool vec, float4 v) {
+    if (vec && type == JX_TYPE_F32) {
+        *reinterpret_cast<float4*>(reinterpret_cast<float*>(p) + i) = v;
+    } else if (vec) {
+        uint2 u;
+        if (type == JX_TYPE_F16)
+            u = make_uint2(half_bits(v.x) | half_bits(v.y) << 16, half_bits(v.z) | half_bits(v.w) << 16);
+        else
+            u = make_uint2(bf16_bits(v.x) | bf16_bits(v.y) << 16, bf16_bits(v.z) | bf16_bits(v.w) << 16);
+        *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p) + i) = u;
+    } else {
+        store1(p, type, i, v.x), store1(p, type, i + 1, v.y), store1(p, type, i + 2, v.z), store1(p, type, i + 3, v.w);
+    }
+}
+
 // 16 consecutive values of a row
 __device__ __forceinline__ void load16(const void* p, int type, int64_t i, bool vec, float (&v)[16]) {
     if (vec && type == JX_TYPE_F32) {
@@ -80,26 +96,122 @@ __device__ __forceinline__ float tanh_fast(float z) {
     return __builtin_copysignf(a < 0.25f ? small : big, z);
 }
 
-// ND signed digits of q in MFMA operand order: lane (h, c) holds dimensions 32 j + 16 h .. + 15 of row c.  qs: the value of
-// one unit of the last digit, NaN where the row has a value that is not finite.
-template <int DT, int ND>
-__device__ __forceinline__ void load_q(const AttendArgs& a, int row, int head, int h, bool valid, v4i (&qd)[ND][DT], float& qs) {
-    constexpr float TOP = ND == 2 ? 127.0f * 128.0f : 127.0f * 16384.0f;
-    float v[DT][16];
-    uint32_t top = 0;
-    const int64_t at = (int64_t)row * a.q_stride + (int64_t)head * a.c.D + 16 * h;
+__device__ __forceinline__ int lane_of(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+__device__ __forceinline__ uint32_t lane_of(uint32_t v, int lane) { return (uint32_t)__builtin_amdgcn_readlane((int)v, lane); }
+__device__ __forceinline__ float lane_of(float v, int lane) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), lane)); }
+
+// (v of the lane 32 below or its own, v of the lane 32 above or its own): one of the two is the other half's.  16: of each 32 lanes
+__device__ __forceinline__ float2 both32(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return make_float2(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float2 both16(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return make_float2(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+// Over the lanes of a row: lane + 32 (and + 16, where 16 lanes hold the rows)
+template <int NR>
+__device__ __forceinline__ float row_max(float v) {
+    const float2 a = both32(v);
+    v = fmaxf(a.x, a.y);
+    if constexpr (NR == 16) {
+        const float2 b = both16(v);
+        v = fmaxf(b.x, b.y);
+    }
+    return v;
+}
+template <int NR>
+__device__ __forceinline__ float row_sum(float v) {
+    const float2 a = both32(v);
+    v = a.x + a.y;
+    if constexpr (NR == 16) {
+        const float2 b = both16(v);
+        v = b.x + b.y;
+    }
+    return v;
+}
+
+typedef float v4f __attribute__((ext_vector_type(4)));
+
+// What differs between a wave that takes 32 rows and one that takes up to 16 (half the registers and arithmetic for the same
+// codes, so twice the waves: the form for single tokens).  col: the lane's row; g: its part of the others' dimension.
+//   result of K Q^T: register x holds token token(x) + 4 g; of V^T P^T: register x of tile i holds dimension DI * i + dim(x) + 4 g
+template <int NR, int DT>
+struct Form;
+template <int DT>
+struct Form<32, DT> {
+    typedef v16i Acc;
+    typedef v16f Out;
+    static constexpr int STEPS = DT, X = 16, TILES = DT, DI = 32, ACCS = 1;  // ACCS: result tiles of 32 tokens
+    static __device__ constexpr int token(int x) { return 8 * (x >> 2) + (x & 3); }
+    static __device__ constexpr int dim(int x) { return 8 * (x >> 2) + (x & 3); }
+    static __device__ __forceinline__ int chunk(int j, int g) { return 2 * j + g; }  // of 16 dimensions
+    static __device__ __forceinline__ int k_at(int j, int g, int col) { return (2 * j + g) * 512 + col * 16; }
+    static __device__ __forceinline__ int v_at(int j, int g, int col) { return (g * 32 * DT + 32 * j + col) * 16; }
+    static __device__ __forceinline__ Acc scores(v4i k, v4i q, Acc c) { return __builtin_amdgcn_mfma_i32_32x32x32_i8(k, q, c, 0, 0, 0); }
+};
+template <int DT>
+struct Form<16, DT> {
+    typedef v4i Acc;
+    typedef v4f Out;
+    static constexpr int STEPS = (DT + 1) / 2, X = 8, TILES = 2 * DT, DI = 16, ACCS = 2;
+    static __device__ constexpr int token(int x) { return 16 * (x >> 2) + (x & 3); }
+    static __device__ constexpr int dim(int x) { return x; }
+    static __device__ __forceinline__ int chunk(int j, int g) { return 4 * j + g; }
+    // (the last step of an odd DT has two chunks: the other lanes read the same ones, against zeros of q)
+    static __device__ __forceinline__ int k_chunk(int j, int g) { return DT % 2 && j == STEPS - 1 ? 4 * j + (g & 1) : 4 * j + g; }
+    static __device__ __forceinline__ Acc scores(v4i k, v4i q, Acc c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(k, q, c, 0, 0, 0); }
+};
+
+template <int NR, int DT>
+using AccOf = typename Form<NR, DT>::Acc;
+template <int NR, int DT, int ND>
+using Scores = AccOf<NR, DT>[ND][Form<NR, DT>::ACCS];
+template <int NR, int DT, int ND>
+using Digits = v4i[ND][Form<NR, DT>::STEPS];
+template <int NR, int DT>
+using Keys = v4i[Form<NR, DT>::ACCS][Form<NR, DT>::STEPS];
+
+// The lane's values of q: the 16 dimensions of chunk(j, g) of its row
+template <int NR, int DT>
+using Raw = float[Form<NR, DT>::STEPS][16];
+template <int NR, int DT>
+__device__ __forceinline__ void load_q(const AttendArgs& a, int row, int head, int g, bool valid, Raw<NR, DT>& v) {
+    typedef Form<NR, DT> F;
+    const int64_t at = (int64_t)row * a.q_stride + (int64_t)head * a.c.D;
 #pragma unroll
-    for (int j = 0; j < DT; ++j) {
-        if (valid) {
-            load16(a.q, a.type, at + 32 * j, a.q_vec, v[j]);
+    for (int j = 0; j < F::STEPS; ++j) {
+        if (valid && F::chunk(j, g) < 2 * DT) {
+            load16(a.q, a.type, at + 16 * F::chunk(j, g), a.q_vec, v[j]);
         } else {
 #pragma unroll
             for (int k = 0; k < 16; ++k) v[j][k] = 0.0f;
         }
+    }
+}
+
+// Byte 0 of four words
+__device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    const uint32_t lo = __builtin_amdgcn_perm(b, a, 0x0C0C0400u), hi = __builtin_amdgcn_perm(d, c, 0x04000C0Cu);
+    return lo | hi;
+}
+
+// ND signed digits of it in MFMA operand order, 127 times the top digit's unit for the row's largest value.  qs: the value of one
+// unit of the last digit, NaN where the row has a value that is not finite.
+//   u = rint(v * TOP / amax) + 64 (1 + 128): added to 1.5 2^23 by the multiply-add that forms it, u is in the low mantissa bits;
+//   its groups of 7 bits are the lower digits + 64, what is above them the top digit.
+template <int NR, int DT, int ND>
+__device__ __forceinline__ void digits(const Raw<NR, DT>& v, Digits<NR, DT, ND>& qd, float& qs) {
+    typedef Form<NR, DT> F;
+    constexpr float TOP = ND == 2 ? 127.0f * 128.0f : 127.0f * 16384.0f;
+    constexpr float MAGIC = 12582912.0f + (ND == 2 ? 64.0f : 64.0f + 64.0f * 128.0f);
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < F::STEPS; ++j)
 #pragma unroll
         for (int k = 0; k < 16; ++k) top = max(top, __float_as_uint(v[j][k]) & 0x7FFFFFFFu);  // orders NaN and infinity last
-    }
     top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
+    if constexpr (NR == 16) top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
     const bool finite = top < 0x7F800000u;
     // rows below 2^-100 count as zero: TOP / amax stays finite
     const bool zero = top < 0x0D800000u;
@@ -107,49 +219,47 @@ __device__ __forceinline__ void load_q(const AttendArgs& a, int row, int head, i
     const float inv = finite && !zero ? TOP / amax : 0.0f;
     qs = !finite ? __uint_as_float(0x7FC00000u) : zero ? 0.0f : amax / TOP;
 #pragma unroll
-    for (int j = 0; j < DT; ++j) {
-        uint32_t w[ND][4] = {};
+    for (int j = 0; j < F::STEPS; ++j)
 #pragma unroll
-        for (int k = 0; k < 16; ++k) {
-            int u = finite ? (int)__builtin_rintf(v[j][k] * inv) : 0;
+        for (int k = 0; k < 16; k += 4) {
+            uint32_t u[4];
 #pragma unroll
-            for (int n = ND - 1; n > 0; --n) {  // last digits first, -64 .. 63
-                const int up = (u + 64) >> 7;
-                w[n][k >> 2] |= (uint32_t)((u - (up << 7)) & 255) << (8 * (k & 3));
-                u = up;
+            for (int i = 0; i < 4; ++i) u[i] = __float_as_uint(__builtin_fmaf(v[j][k + i], inv, MAGIC));
+#pragma unroll
+            for (int n = ND - 1; n > 0; --n) {
+                // a byte d + 64 (0 .. 127) -> d: bit 6 flipped, and the sign where it is then set
+                const uint32_t y = (pack4(u[0], u[1], u[2], u[3]) & 0x7F7F7F7Fu) ^ 0x40404040u;
+                qd[n][j][k >> 2] = (int)(y | (y & 0x40404040u) << 1);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) u[i] >>= 7;
             }
-            w[0][k >> 2] |= (uint32_t)(u & 255) << (8 * (k & 3));
+            qd[0][j][k >> 2] = (int)pack4(u[0], u[1], u[2], u[3]);
         }
-#pragma unroll
-        for (int n = 0; n < ND; ++n) qd[n][j] = v4i{(int)w[n][0], (int)w[n][1], (int)w[n][2], (int)w[n][3]};
-    }
 }
 
-// What a wave carries for its 32 rows.
-template <int DT>
+// What a wave carries for its rows.
+template <int NR, int DT>
 struct Carry {
-    v16f o[DT];
-    float m, l;  // of the lane's row: reference maximum (log2), sum of the weights of this lane half
+    typename Form<NR, DT>::Out o[Form<NR, DT>::TILES];
+    float m, l;  // of the lane's row: reference maximum (log2), sum of the weights of the lane's tokens
     float R;     // largest scale of V's blocks so far
 };
 
-template <int DT>
-__device__ __forceinline__ void carry_init(Carry<DT>& s) {
+template <int NR, int DT>
+__device__ __forceinline__ void carry_init(Carry<NR, DT>& s) {
 #pragma unroll
-    for (int i = 0; i < DT; ++i)
-#pragma unroll
-        for (int k = 0; k < 16; ++k) s.o[i][k] = 0.0f;
+    for (auto& o : s.o) o = typename Form<NR, DT>::Out{};
     s.m = -__builtin_inff();
     s.l = 0.0f;
     s.R = 0.0f;
 }
 
-template <int DT>
-__device__ __forceinline__ void carry_scale(Carry<DT>& s, float f) {
+template <int NR, int DT>
+__device__ __forceinline__ void carry_scale(Carry<NR, DT>& s, float f) {
 #pragma unroll
-    for (int i = 0; i < DT; ++i)
+    for (auto& o : s.o)
 #pragma unroll
-        for (int k = 0; k < 16; ++k) s.o[i][k] *= f;
+        for (int k = 0; k < (NR == 32 ? 16 : 4); ++k) o[k] *= f;
 }
 
 __device__ __forceinline__ h8 codes_to_half(uint32_t w0, uint32_t w1) {
@@ -157,50 +267,60 @@ __device__ __forceinline__ h8 codes_to_half(uint32_t w0, uint32_t w1) {
     return cvt8(w0, w1, 0xFFFFFFFFu, 0x80808080u, one, bias);  // 1024 + (code + 128) - 1152
 }
 
-// One block of 32 tokens from t0 on.  lo / hi: the lane's row sees tokens lo .. hi - 1 (masked: whether to look).
-template <int DT, int ND, bool EXT>
-__device__ __forceinline__ void tile(Carry<DT>& s, const AttendArgs& a, const v4i (&qd)[ND][DT], float qs, float slope, int pos,
-                                     const v4i (&kc)[DT], const v4i (&vc)[DT], float ks, float vs, int t0, int h, int lo, int hi,
-                                     bool masked) {
-    v16i acc[ND];
+// S^T of one block of 32 tokens, digit by digit.  kc: [result tile][step]
+template <int NR, int DT, int ND>
+__device__ __forceinline__ void scores(Scores<NR, DT, ND>& acc, const Digits<NR, DT, ND>& qd,
+                                       const Keys<NR, DT>& kc) {
+    typedef Form<NR, DT> F;
 #pragma unroll
-    for (int n = 0; n < ND; ++n) {
-        acc[n] = v16i{};
+    for (int n = 0; n < ND; ++n)
 #pragma unroll
-        for (int j = 0; j < DT; ++j) acc[n] = __builtin_amdgcn_mfma_i32_32x32x32_i8(kc[j], qd[n][j], acc[n], 0, 0, 0);
-    }
-    float x[16];
+        for (int t = 0; t < F::ACCS; ++t) acc[n][t] = typename F::Acc{};
+#pragma unroll
+    for (int j = 0; j < F::STEPS; ++j)
+#pragma unroll
+        for (int t = 0; t < F::ACCS; ++t)
+#pragma unroll
+            for (int n = 0; n < ND; ++n) acc[n][t] = F::scores(kc[t][j], qd[n][j], acc[n][t]);
+}
+
+// The rest of the block, whose tokens begin at t0.  lo / hi: the lane's row sees tokens lo .. hi - 1 (masked: whether to look).
+template <int NR, int DT, int ND, bool EXT>
+__device__ __forceinline__ void weigh(Carry<NR, DT>& s, const AttendArgs& a, const Scores<NR, DT, ND>& acc,
+                                      float qs, float slope, int pos, const v4i (&vc)[DT], float ks, float vs, int t0, int g, int lo,
+                                      int hi, bool masked) {
+    typedef Form<NR, DT> F;
+    constexpr int X = F::X, PER = X / F::ACCS;
+    float x[X];
     const float c = qs * ks * (EXT ? a.scale : a.scale2);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < X; ++i) {
+        const int t = i / PER, k = i % PER;
         // |acc| <= 127 * 127 * 256: two digits fit an int32
         if constexpr (ND == 2)
-            x[i] = (float)(acc[0][i] * 128 + acc[1][i]) * c;
+            x[i] = (float)(acc[0][t][k] * 128 + acc[1][t][k]) * c;
         else
-            x[i] = __builtin_fmaf((float)acc[0][i], 16384.0f, (float)(acc[1][i] * 128 + acc[2][i])) * c;
+            x[i] = __builtin_fmaf((float)acc[0][t][k], 16384.0f, (float)(acc[1][t][k] * 128 + acc[2][t][k])) * c;
     }
     if constexpr (EXT) {
         if (a.cap > 0.0f) {
             const float inv = 1.0f / a.cap;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) x[i] = a.cap * tanh_fast(x[i] * inv);
+            for (int i = 0; i < X; ++i) x[i] = a.cap * tanh_fast(x[i] * inv);
         }
-        const float d0 = (float)(t0 + 4 * h - pos);
+        const float d0 = (float)(t0 + 4 * g - pos);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = __builtin_fmaf(slope, d0 + (float)(8 * (i >> 2) + (i & 3)), x[i]) * LOG2E;
+        for (int i = 0; i < X; ++i) x[i] = __builtin_fmaf(slope, d0 + (float)F::token(i), x[i]) * LOG2E;
     }
+    const int l0 = lo - t0 - 4 * g, h0 = hi - t0 - 4 * g;
     if (masked) {
-        const int l0 = lo - t0 - 4 * h, h0 = hi - t0 - 4 * h;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int t = 8 * (i >> 2) + (i & 3);
-            x[i] = t >= l0 && t < h0 ? x[i] : -__builtin_inff();
-        }
+        for (int i = 0; i < X; ++i) x[i] = F::token(i) >= l0 && F::token(i) < h0 ? x[i] : -__builtin_inff();
     }
     float top = x[0];
 #pragma unroll
-    for (int i = 1; i < 16; ++i) top = fmaxf(top, x[i]);
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    for (int i = 1; i < X; ++i) top = fmaxf(top, x[i]);
+    top = row_max<NR>(top);
     if (__any(top > s.m + LAG)) {
         const float m = fmaxf(s.m, top);
         const float f = m == s.m ? 1.0f : __builtin_amdgcn_exp2f(s.m - m);
@@ -217,45 +337,188 @@ __device__ __forceinline__ void tile(Carry<DT>& s, const AttendArgs& a, const v4
     const float ref = s.m == -__builtin_inff() ? (float)-OFF : s.m - (float)OFF;
     float sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < X; ++i) {
         const float p = __builtin_amdgcn_exp2f(x[i] - ref);
         sum += p;
         x[i] = p * vr;
     }
     if (masked) {  // nothing of a NaN scale reaches a row that does not see the block
-        const int l0 = lo - t0 - 4 * h, h0 = hi - t0 - 4 * h;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int t = 8 * (i >> 2) + (i & 3);
-            x[i] = t >= l0 && t < h0 ? x[i] : 0.0f;
-        }
+        for (int i = 0; i < X; ++i) x[i] = F::token(i) >= l0 && F::token(i) < h0 ? x[i] : 0.0f;
     }
     s.l += sum;
-    // token 8 a + 4 h + b is register 4 a + b here and byte 8 (a & 1) + 4 (a >> 1) + b of V
-    h8 p0, p1, e0, e1;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        p0[i] = (_Float16)x[i], p0[4 + i] = (_Float16)x[8 + i];
-        p1[i] = (_Float16)x[4 + i], p1[4 + i] = (_Float16)x[12 + i];
-    }
-    if constexpr (ND == 3) {  // the weights' remainders: 22 bits in all
+    if constexpr (NR == 32) {
+        // token 8 a + 4 g + b is register 4 a + b here and byte 8 (a & 1) + 4 (a >> 1) + b of V
+        h8 p0, p1, e0, e1;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            e0[i] = (_Float16)(x[i] - (float)p0[i]), e0[4 + i] = (_Float16)(x[8 + i] - (float)p0[4 + i]);
-            e1[i] = (_Float16)(x[4 + i] - (float)p1[i]), e1[4 + i] = (_Float16)(x[12 + i] - (float)p1[4 + i]);
+            p0[i] = (_Float16)x[i], p0[4 + i] = (_Float16)x[8 + i];
+            p1[i] = (_Float16)x[4 + i], p1[4 + i] = (_Float16)x[12 + i];
         }
-    }
+        if constexpr (ND == 3) {  // the weights' remainders: 22 bits in all
 #pragma unroll
-    for (int i = 0; i < DT; ++i) {
-        const h8 v0 = codes_to_half((uint32_t)vc[i][0], (uint32_t)vc[i][1]);
-        const h8 v1 = codes_to_half((uint32_t)vc[i][2], (uint32_t)vc[i][3]);
-        s.o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v0, p0, s.o[i], 0, 0, 0);
-        s.o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v1, p1, s.o[i], 0, 0, 0);
+            for (int i = 0; i < 4; ++i) {
+                e0[i] = (_Float16)(x[i] - (float)p0[i]), e0[4 + i] = (_Float16)(x[8 + i] - (float)p0[4 + i]);
+                e1[i] = (_Float16)(x[4 + i] - (float)p1[i]), e1[4 + i] = (_Float16)(x[12 + i] - (float)p1[4 + i]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < DT; ++i) {
+            const h8 v0 = codes_to_half((uint32_t)vc[i][0], (uint32_t)vc[i][1]);
+            const h8 v1 = codes_to_half((uint32_t)vc[i][2], (uint32_t)vc[i][3]);
+            s.o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v0, p0, s.o[i], 0, 0, 0);
+            s.o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v1, p1, s.o[i], 0, 0, 0);
+            if constexpr (ND == 3) {
+                s.o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v0, e0, s.o[i], 0, 0, 0);
+                s.o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v1, e1, s.o[i], 0, 0, 0);
+            }
+        }
+    } else {
+        // registers 0 .. 3 are tokens 4 g + b, 4 .. 7 tokens 16 + 4 g + b: of a piece (h, d) of V the eight bytes from
+        // 8 (g >> 1) on, h = g & 1.  The lane loaded all 16 bytes of piece h of dimension 32 i + 16 (g >> 1) + col: the
+        // halves of the wave exchange what belongs to the other's 16 dimensions.
+        h8 p, e;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p[i] = (_Float16)x[i];
         if constexpr (ND == 3) {
-            s.o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v0, e0, s.o[i], 0, 0, 0);
-            s.o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v1, e1, s.o[i], 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) e[i] = (_Float16)(x[i] - (float)p[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < DT; ++i) {
+            const auto r0 = __builtin_amdgcn_permlane32_swap((uint32_t)vc[i][0], (uint32_t)vc[i][2], false, false);
+            const auto r1 = __builtin_amdgcn_permlane32_swap((uint32_t)vc[i][1], (uint32_t)vc[i][3], false, false);
+            const h8 v0 = codes_to_half(r0[0], r1[0]), v1 = codes_to_half(r0[1], r1[1]);
+            s.o[2 * i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, p, s.o[2 * i], 0, 0, 0);
+            s.o[2 * i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, p, s.o[2 * i + 1], 0, 0, 0);
+            if constexpr (ND == 3) {
+                s.o[2 * i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, e, s.o[2 * i], 0, 0, 0);
+                s.o[2 * i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, e, s.o[2 * i + 1], 0, 0, 0);
+            }
         }
     }
+}
+
+// The blocks of up to 64 tiles, one per lane
+struct Blocks {
+    int k, v;       // block numbers
+    float ks, vs;   // scales
+};
+__device__ __forceinline__ int page_of(const AttendArgs& a, int slot, int tile, bool valid) {
+    return valid ? a.c.table[(int64_t)slot * a.c.max_pages + (tile >> a.c.blocks_shift)] : 0;
+}
+__device__ __forceinline__ Blocks blocks_of(const AttendArgs& a, int kvh, int page, int tile, bool valid) {
+    Blocks b = {0, 0, 0.0f, 0.0f};
+    if (valid) {
+        const bool bad = page < 0 || page >= a.c.n_pages;
+        page = bad ? 0 : page;
+        const int blk = tile & ((1 << a.c.blocks_shift) - 1);
+        b.k = a.c.block_index(page, 0, kvh, blk);
+        b.v = a.c.block_index(page, 1, kvh, blk);
+        b.ks = a.c.scales[b.k];
+        b.vs = a.c.scales[b.v];
+        if (bad) {
+            b.ks = b.vs = __uint_as_float(0x7FC00000u);
+            atomicOr(a.c.status, JX_KV_BAD_PAGE);
+        }
+    }
+    return b;
+}
+
+// A wave's rows against `count` tiles, first + i * step.  Everything that waits for memory is asked for as early as its address is
+// known: pages, then q, then scales and the first block, and q's digits are formed while that arrives.  In the loop a
+// block's registers are loaded again as soon as its products are issued: the next K arrives behind the weights and the
+// product with V, the next V behind the next scores.  (Two full sets of registers spilled at 128 dimensions.)
+template <int NR, int DT, int ND, bool EXT, bool ONCE>
+__device__ __forceinline__ void attend_tiles(Carry<NR, DT>& cy, const AttendArgs& a, const KvSeq& s, int kvh, int row, int head, bool valid,
+                                             int pos, int first, int step, int count, int whole_lo, int whole_hi) {
+    typedef Form<NR, DT> F;
+    const int lane = threadIdx.x & 63, g = lane / NR, col = lane % NR;
+    const int hi = a.causal ? min(s.len, pos + 1) : s.len, lo = a.window ? max(0, pos - a.window + 1) : 0;
+    const int64_t bytes = (int64_t)KV_BLOCK * 32 * DT;
+    auto ld = [](const int8_t* p) {  // (blocks that one wave alone reads: without a place in the caches)
+        const v4i* q = reinterpret_cast<const v4i*>(p);
+        return ONCE ? __builtin_nontemporal_load(q) : *q;
+    };
+    Blocks bl;
+    Keys<NR, DT> k;
+    v4i v[DT];
+    auto fetch_k = [&](int i) {
+        const int8_t* p = a.c.codes + lane_of(bl.k, i) * bytes;
+#pragma unroll
+        for (int j = 0; j < F::STEPS; ++j)
+#pragma unroll
+            for (int t = 0; t < F::ACCS; ++t) {
+                if constexpr (NR == 32)
+                    k[t][j] = ld(p + F::k_at(j, g, col));
+                else
+                    k[t][j] = ld(p + F::k_chunk(j, g) * 512 + (16 * t + col) * 16);
+            }
+    };
+    auto fetch_v = [&](int i) {
+        const int8_t* p = a.c.codes + lane_of(bl.v, i) * bytes;
+#pragma unroll
+        for (int j = 0; j < DT; ++j) {
+            if constexpr (NR == 32)
+                v[j] = ld(p + F::v_at(j, g, col));
+            else
+                v[j] = ld(p + ((g & 1) * 32 * DT + 32 * j + 16 * (g >> 1) + col) * 16);
+        }
+    };
+    int page = page_of(a, s.slot, first + lane * step, lane < count);
+    Raw<NR, DT> raw;
+    load_q<NR, DT>(a, row, head, g, valid, raw);
+    const float slope = EXT && a.alibi ? a.alibi[head] : 0.0f;
+    bl = blocks_of(a, kvh, page, first + lane * step, lane < count);
+    if (count > 0) {
+        fetch_k(0);
+        fetch_v(0);
+    }
+    Digits<NR, DT, ND> qd;
+    float qs;
+    digits<NR, DT, ND>(raw, qd, qs);
+    for (int b0 = 0; b0 < count; b0 += 64) {
+        const int n = min(64, count - b0);
+        if (b0) {
+            const int mine = first + (b0 + lane) * step;
+            bl = blocks_of(a, kvh, page_of(a, s.slot, mine, lane < n), mine, lane < n);
+            fetch_k(0);
+            fetch_v(0);
+        }
+        for (int i = 0; i < n; ++i) {
+            Scores<NR, DT, ND> acc;
+            scores<NR, DT, ND>(acc, qd, k);
+            if (i + 1 < n) fetch_k(i + 1);
+            const int t0 = (first + (b0 + i) * step) * KV_BLOCK;
+            weigh<NR, DT, ND, EXT>(cy, a, acc, qs, slope, pos, v, lane_of(bl.ks, i), lane_of(bl.vs, i), t0, g, lo, hi,
+                                   t0 < whole_lo || t0 + KV_BLOCK > whole_hi);
+            if (i + 1 < n) fetch_v(i + 1);
+        }
+    }
+}
+
+// The sums of the lane's row as floats at o (16-byte aligned), times f
+template <int NR, int DT>
+__device__ __forceinline__ void put_sums(const Carry<NR, DT>& cy, float* o, int g, float f) {
+    typedef Form<NR, DT> F;
+#pragma unroll
+    for (int i = 0; i < F::TILES; ++i)
+#pragma unroll
+        for (int k = 0; k < (NR == 32 ? 16 : 4); k += 4)
+            *reinterpret_cast<float4*>(o + F::DI * i + F::dim(k) + 4 * g) =
+                make_float4(cy.o[i][k] * f, cy.o[i][k + 1] * f, cy.o[i][k + 2] * f, cy.o[i][k + 3] * f);
+}
+// The same as the call's type at element `at` of out
+template <int NR, int DT>
+__device__ __forceinline__ void put_out(const Carry<NR, DT>& cy, const AttendArgs& a, int64_t at, int g, float f) {
+    typedef Form<NR, DT> F;
+#pragma unroll
+    for (int i = 0; i < F::TILES; ++i)
+#pragma unroll
+        for (int k = 0; k < (NR == 32 ? 16 : 4); k += 4) {
+            const float4 y = make_float4(cy.o[i][k] * f, cy.o[i][k + 1] * f, cy.o[i][k + 2] * f, cy.o[i][k + 3] * f);
+            store4(a.out, a.type, at + F::DI * i + F::dim(k) + 4 * g, a.out_vec, y);
+        }
 }
 
 // The tiles of 32 tokens that a row tile of a sequence sees, and how they are divided.
@@ -283,10 +546,10 @@ __host__ __device__ constexpr int waves_of(int dt) { return dt <= 4 ? 8 : 4; }
 
 // blockIdx.x = ((sequence * splits + split) * row_tiles + row tile) * H + kv head.  The waves of a workgroup take the tiles of
 // its split in turn and join in LDS.
-template <int DT, int ND, bool EXT>
+template <int NR, int DT, int ND, bool EXT>
 __global__ __launch_bounds__(64 * waves_of(DT)) void k_attend(const AttendArgs a) {
     extern __shared__ float lds[];
-    const int W = blockDim.x >> 6, wave = threadIdx.x >> 6, lane = threadIdx.x & 63, h = lane >> 5, col = lane & 31;
+    const int W = blockDim.x >> 6, wave = threadIdx.x >> 6, lane = threadIdx.x & 63, gl = lane / NR, col = lane % NR;
     int item = blockIdx.x;
     const int kvh = item % a.c.H;
     item /= a.c.H;
@@ -295,81 +558,28 @@ __global__ __launch_bounds__(64 * waves_of(DT)) void k_attend(const AttendArgs a
     const int split = item % a.splits, seq = item / a.splits;
     const int failed = *a.c.status;
     const KvSeq s = kv_seq(a.c, a.b, seq);
-    const int rows = s.n * a.G, r0 = rt * 32;
+    const int rows = s.n * a.G, r0 = rt * NR;
     if (r0 >= rows) return;
-    const int nr = min(32, rows - r0);
+    const int nr = min(NR, rows - r0);
     const Range g = range_of(a, s, r0, nr);
     if (split >= g.n) return;
     const int r = r0 + min(col, nr - 1), head = kvh * a.G + r % a.G, row = s.row0 + r / a.G, pos = g.base + r / a.G;
-    const int hi = a.causal ? min(s.len, pos + 1) : s.len, lo = a.window ? max(0, pos - a.window + 1) : 0;
     // tiles that every row sees whole need no mask: hi of the first row, lo of the last
     const int p0 = g.base + r0 / a.G, p1 = g.base + (r0 + nr - 1) / a.G;
     const int whole_hi = a.causal ? min(s.len, p0 + 1) : s.len, whole_lo = a.window ? max(0, p1 - a.window + 1) : 0;
-
-    v4i qd[ND][DT];
-    float qs;
-    load_q<DT, ND>(a, row, head, h, col < nr, qd, qs);
-    const float slope = EXT && a.alibi ? a.alibi[head] : 0.0f;
-    Carry<DT> cy;
+    Carry<NR, DT> cy;
     carry_init(cy);
-
     const int first = g.begin + split * g.per + wave, end = g.begin + min(g.tiles, (split + 1) * g.per);
-    const int mine = first < end ? (end - first + W - 1) / W : 0;
-    const int64_t bytes = (int64_t)KV_BLOCK * a.c.D;
-    for (int b0 = 0; b0 < mine; b0 += 64) {
-        // the lane's tile of the next 64: its blocks and scales
-        int kb = 0, vb = 0;
-        float ks = 0.0f, vs = 0.0f;
-        if (b0 + lane < mine) {
-            const int t = first + (b0 + lane) * W;
-            int page = a.c.table[(int64_t)s.slot * a.c.max_pages + (t >> a.c.blocks_shift)];
-            const bool bad = page < 0 || page >= a.c.n_pages;
-            page = bad ? 0 : page;
-            const int blk = t & ((1 << a.c.blocks_shift) - 1);
-            kb = a.c.block_index(page, 0, kvh, blk);
-            vb = a.c.block_index(page, 1, kvh, blk);
-            ks = a.c.scales[kb];
-            vs = a.c.scales[vb];
-            if (bad) {
-                ks = vs = __uint_as_float(0x7FC00000u);
-                atomicOr(a.c.status, JX_KV_BAD_PAGE);
-            }
-        }
-        const int count = min(64, mine - b0);
-        v4i kc[DT], vc[DT], kn[DT], vn[DT];
-        auto fetch = [&](int i, v4i(&k)[DT], v4i(&v)[DT]) {
-            const int8_t* kp = a.c.codes + __builtin_amdgcn_readlane(kb, i) * bytes + lane * 16;
-            const int8_t* vp = a.c.codes + __builtin_amdgcn_readlane(vb, i) * bytes + h * (16 * a.c.D) + col * 16;
-#pragma unroll
-            for (int j = 0; j < DT; ++j) k[j] = *reinterpret_cast<const v4i*>(kp + j * 1024);
-#pragma unroll
-            for (int j = 0; j < DT; ++j) v[j] = *reinterpret_cast<const v4i*>(vp + j * 512);
-        };
-        fetch(0, kc, vc);
-        for (int i = 0; i < count; ++i) {
-            if (i + 1 < count) fetch(i + 1, kn, vn);
-            const int t0 = (first + (b0 + i) * W) * KV_BLOCK;
-            const float ki = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks), i));
-            const float vi = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs), i));
-            tile<DT, ND, EXT>(cy, a, qd, qs, slope, pos, kc, vc, ki, vi, t0, h, lo, hi, t0 < whole_lo || t0 + KV_BLOCK > whole_hi);
-#pragma unroll
-            for (int j = 0; j < DT; ++j) kc[j] = kn[j], vc[j] = vn[j];
-        }
-    }
+    attend_tiles<NR, DT, ND, EXT, false>(cy, a, s, kvh, row, head, col < nr, pos, first, W, first < end ? (end - first + W - 1) / W : 0,
+                                         whole_lo, whole_hi);
 
     // the waves' sums: [W][rows_cap][D], then [W][rows_cap][2] with the maximum and the sum of weights
     float* so = lds;
     float* sm = lds + (size_t)W * a.rows_cap * a.c.D;
-    cy.l += __shfl_xor(cy.l, 32, 64);
+    cy.l = row_sum<NR>(cy.l);
     if (col < nr) {
-        float* o = so + ((size_t)wave * a.rows_cap + col) * a.c.D;
-#pragma unroll
-        for (int i = 0; i < DT; ++i)
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-                *reinterpret_cast<float4*>(o + 32 * i + 8 * k + 4 * h) =
-                    make_float4(cy.o[i][4 * k] * cy.R, cy.o[i][4 * k + 1] * cy.R, cy.o[i][4 * k + 2] * cy.R, cy.o[i][4 * k + 3] * cy.R);
-        if (h == 0) {
+        put_sums(cy, so + ((size_t)wave * a.rows_cap + col) * a.c.D, gl, cy.R);
+        if (gl == 0) {
             sm[(wave * a.rows_cap + col) * 2] = cy.m;
             sm[(wave * a.rows_cap + col) * 2 + 1] = cy.l;
         }
@@ -393,14 +603,94 @@ __global__ __launch_bounds__(64 * waves_of(DT)) void k_attend(const AttendArgs a
             if (failed) y = __uint_as_float(0x7FC00000u);
             store1(a.out, a.type, (int64_t)orow * a.out_stride + (int64_t)ohead * D + d, y);
         } else {
-            const int64_t at = ((int64_t)orow * a.heads + ohead) * a.splits + split;
+            const int64_t at = (int64_t)blockIdx.x * a.rows_cap + rr;
             a.part_o[at * D + d] = o;
             if (d == 0) a.part_ml[at * 2] = m, a.part_ml[at * 2 + 1] = l;
         }
     }
 }
 
-// Rows that were divided: their splits' sums joined.  A wave per row; grid as k_attend's without the splits.
+// The row `rr` of n partials, joined and stored, by W = 4 waves of a workgroup or by each wave alone (1).  part(i): number of
+// the i-th partial.  A load takes 16 bytes per lane: 64 lanes hold `subs` rows of partials, and eight loads are in flight.
+constexpr int FLIGHT = 8;
+template <int W, typename F>
+__device__ __forceinline__ void join_row(const AttendArgs& a, int n, int rr, int64_t to, int failed, F part) {
+    __shared__ float so[4][256], sl[32], sm[32];
+    const int lane = threadIdx.x & 63, wave = W == 1 ? 0 : threadIdx.x >> 6, D = a.c.D;
+    const int width = D <= 32 ? 8 : D <= 64 ? 16 : D <= 128 ? 32 : 64, subs = 64 / width, sub = lane / width, at = lane % width;
+    const bool in = 4 * at < D;
+    float m = -__builtin_inff(), l = 0.0f;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int b0 = 0; b0 < n; b0 += FLIGHT * W * subs) {
+        float2 ml[FLIGHT];
+        float4 v[FLIGHT];
+#pragma unroll
+        for (int u = 0; u < FLIGHT; ++u) {
+            const int i = b0 + (u * W + wave) * subs + sub;
+            const int64_t p = part(min(i, n - 1)) * a.rows_cap + rr;
+            ml[u] = reinterpret_cast<const float2*>(a.part_ml)[p];
+            v[u] = *reinterpret_cast<const float4*>(a.part_o + p * D + (in ? 4 * at : 0));
+            if (i >= n) ml[u] = make_float2(-__builtin_inff(), 0.0f);
+        }
+        float top = m;
+#pragma unroll
+        for (int u = 0; u < FLIGHT; ++u) top = fmaxf(top, ml[u].x);
+        const float old = m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
+        m = top;
+        l *= old;
+        o.x *= old, o.y *= old, o.z *= old, o.w *= old;
+#pragma unroll
+        for (int u = 0; u < FLIGHT; ++u) {
+            if (b0 + (u * W + wave) * subs + sub >= n) continue;
+            const float f = ml[u].x == m ? 1.0f : __builtin_amdgcn_exp2f(ml[u].x - m);
+            l = __builtin_fmaf(f, ml[u].y, l);
+            o.x = __builtin_fmaf(f, v[u].x, o.x), o.y = __builtin_fmaf(f, v[u].y, o.y);
+            o.z = __builtin_fmaf(f, v[u].z, o.z), o.w = __builtin_fmaf(f, v[u].w, o.w);
+        }
+    }
+    if constexpr (W > 1) {
+        if (at == 0) sl[wave * subs + sub] = l, sm[wave * subs + sub] = m;
+    }
+    // the rows of a wave add up in its lanes first
+    float top = m;
+    for (int w = width; w < 64; w <<= 1) top = fmaxf(top, __shfl_xor(top, w, 64));
+    const float f = m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
+    o.x *= f, o.y *= f, o.z *= f, o.w *= f;
+    l *= f;
+    for (int w = width; w < 64; w <<= 1) {
+        o.x += __shfl_xor(o.x, w, 64), o.y += __shfl_xor(o.y, w, 64);
+        o.z += __shfl_xor(o.z, w, 64), o.w += __shfl_xor(o.w, w, 64);
+        l += __shfl_xor(l, w, 64);
+    }
+    if constexpr (W == 1) {
+        const float z = failed ? __uint_as_float(0x7FC00000u) : l == 0.0f ? 0.0f : 1.0f / l;
+        if (sub == 0 && in) store4(a.out, a.type, to + 4 * at, a.out_vec, make_float4(o.x * z, o.y * z, o.z * z, o.w * z));
+        return;
+    }
+    if (sub == 0 && in) *reinterpret_cast<float4*>(&so[wave][4 * at]) = o;
+    __syncthreads();
+    for (int d = threadIdx.x; d < D; d += 256) {
+        float most = -__builtin_inff();
+        for (int i = 0; i < 4 * subs; ++i) most = fmaxf(most, sm[i]);
+        float y = 0.0f, z = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            float mw = -__builtin_inff();
+            for (int i = 0; i < subs; ++i) {
+                const float mi = sm[w * subs + i];
+                mw = fmaxf(mw, mi);
+                z = __builtin_fmaf(mi == most ? 1.0f : __builtin_amdgcn_exp2f(mi - most), sl[w * subs + i], z);
+            }
+            y = __builtin_fmaf(mw == most ? 1.0f : __builtin_amdgcn_exp2f(mw - most), so[w][d], y);
+        }
+        y = z == 0.0f ? 0.0f : y / z;
+        if (failed) y = __uint_as_float(0x7FC00000u);
+        store1(a.out, a.type, to + d, y);
+    }
+}
+
+// Rows that k_attend divided.  blockIdx.x as there without the splits, blockIdx.y = row of the row tile.
+template <int NR>
 __global__ __launch_bounds__(256) void k_attend_join(const AttendArgs a) {
     int item = blockIdx.x;
     const int kvh = item % a.c.H;
@@ -408,45 +698,232 @@ __global__ __launch_bounds__(256) void k_attend_join(const AttendArgs a) {
     const int rt = item % a.row_tiles, seq = item / a.row_tiles;
     const int failed = *a.c.status;
     const KvSeq s = kv_seq(a.c, a.b, seq);
-    const int rows = s.n * a.G, r0 = rt * 32;
-    if (r0 >= rows) return;
-    const int nr = min(32, rows - r0);
-    const Range g = range_of(a, s, r0, nr);
+    const int rows = s.n * a.G, r = rt * NR + blockIdx.y;
+    if (r >= rows) return;
+    const Range g = range_of(a, s, rt * NR, min(NR, rows - rt * NR));
     if (g.n == 1) return;
-    const int lane = threadIdx.x & 63, D = a.c.D;
-    for (int rr = threadIdx.x >> 6; rr < nr; rr += blockDim.x >> 6) {
-        const int row = s.row0 + (r0 + rr) / a.G, head = kvh * a.G + (r0 + rr) % a.G;
-        const int64_t at = ((int64_t)row * a.heads + head) * a.splits;
-        float m = -__builtin_inff();
-        for (int i = 0; i < g.n; ++i) m = fmaxf(m, a.part_ml[(at + i) * 2]);
-        float o[4] = {0.0f, 0.0f, 0.0f, 0.0f}, l = 0.0f;
-        for (int i = 0; i < g.n; ++i) {
-            const float mi = a.part_ml[(at + i) * 2];
-            const float f = mi == m ? 1.0f : __builtin_amdgcn_exp2f(mi - m);
-            l = __builtin_fmaf(f, a.part_ml[(at + i) * 2 + 1], l);
+    const int64_t to = (int64_t)(s.row0 + r / a.G) * a.out_stride + (int64_t)(kvh * a.G + r % a.G) * a.c.D;
+    join_row<4>(a, g.n, blockIdx.y, to, failed,
+             [&](int i) { return (((int64_t)seq * a.splits + i) * a.row_tiles + rt) * a.c.H + kvh; });
+}
+
+// ---------------------------------------------------------------- few rows: the tiles of the whole batch in equal shares
+
+// Every (sequence, kv head) has its tiles one behind the other in one long line, sequences in the batch's order; wave w of
+// the launch takes the places w * per .. of the line.  What a wave has of a sequence and head that others share goes to
+// LDS; the waves of a workgroup join what belongs together there, and only what workgroups share becomes a partial
+// in memory, numbered by the first of the workgroup's waves that has a part: 2 w + 1 where it begins the sequence
+// and head, 2 w where it continues one.  (group = 1: every wave's part goes to memory.)
+// To begin a sequence and head (its pages, scales and q arrive one behind the other) costs about as much as START tiles:
+// 0 / 2 / 4 of them: 62 / 55 / 53 us for 64 sequences of 150 to 8000 tokens (273 MB).
+constexpr int START = 4;
+struct Line {
+    KvSeq s;        // of the lane's sequence (chunk + lane)
+    int tiles;      // of its line per head: START and its tiles, none if it has no rows
+    uint32_t end;   // places of the chunk's sequences up to this one, all heads
+};
+__device__ __forceinline__ Line line_of(const AttendArgs& a, int chunk) {
+    const int lane = threadIdx.x & 63, i = chunk + lane;
+    Line n;
+    n.s = KvSeq{0, 0, 0, 0};
+    n.tiles = 0;
+    if (i < a.b.n_seqs) {
+        n.s = kv_seq(a.c, a.b, i);
+        if (n.s.n > 0) n.tiles = START + range_of(a, n.s, 0, n.s.n * a.G).tiles;
+    }
+    n.end = (uint32_t)n.tiles * a.c.H;
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (lane + 64 * k < D) o[k] = __builtin_fmaf(f, a.part_o[(at + i) * D + lane + 64 * k], o[k]);
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t y = (uint32_t)__shfl_up((int)n.end, o, 64);
+        if (lane >= o) n.end += y;
+    }
+    return n;
+}
+constexpr int MIN_TILES = 2;  // of a share
+// Waves of a SIMD that the registers of k_attend_stream leave room for (and that it is compiled for).  With 16 rows three
+// would fit at 128 dimensions, but more loads in flight read slower: 63 us against 50 for 131000 tokens.
+__host__ __device__ constexpr int stream_occupancy(int nr, int dt) { return nr == 32 && dt > 4 ? 1 : 2; }
+// LDS of a workgroup that joins its waves' parts
+inline size_t stream_lds(int rows, int D) { return sizeof(float) * (size_t)8 * rows * (D + 2); }
+__device__ __forceinline__ int per_wave(const AttendArgs& a, uint32_t total) {
+    return max(MIN_TILES, (int)((total + a.waves - 1) / a.waves));
+}
+
+// What a wave left in LDS: a part of a sequence and head (slot 0: continued from the wave before, slot 1: begun)
+struct Part {
+    int rows, row0, kvh;  // rows 0: none
+    bool ends;            // with the last of its tiles
+};
+
+template <int NR, int DT, int ND, bool EXT>
+__global__ __launch_bounds__(256, stream_occupancy(NR, DT)) void k_attend_stream(const AttendArgs a) {
+    extern __shared__ float lds[];  // [4 waves][2 slots][rows_cap][D], then [..][rows_cap][2]
+    __shared__ Part parts[4][2];
+    __shared__ Line lines[4][64];   // (kept here: the registers are needed for the tiles)
+    const int lane = threadIdx.x & 63, gl = lane / NR, col = lane % NR, wave = threadIdx.x >> 6, D = a.c.D;
+    const int w = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + wave);
+    const int failed = *a.c.status;
+    float* sums = lds;
+    float2* stats = reinterpret_cast<float2*>(lds + (size_t)8 * a.rows_cap * D);
+    if (lane < 2) parts[wave][lane].rows = 0;
+    uint32_t total, chunk_end;  // places of the line; of the chunk in `lines`
+    {
+        const Line n = line_of(a, 0);
+        lines[wave][lane] = n;
+        total = chunk_end = lane_of(n.end, 63);
+        for (int c = 64; c < a.b.n_seqs; c += 64) total += lane_of(line_of(a, c).end, 63);
+    }
+    const int per = per_wave(a, total);
+    uint32_t at = (uint32_t)w * per;
+    const uint32_t to = min(total, at + per);
+    uint32_t base = 0;  // places before the chunk
+    int chunk = 0;
+    while (at < to) {
+        while (at - base >= chunk_end) {
+            base += chunk_end;
+            chunk += 64;
+            const Line n = line_of(a, chunk);
+            lines[wave][lane] = n;
+            chunk_end = lane_of(n.end, 63);
         }
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (lane + 64 * k < D) {
-                float y = l == 0.0f ? 0.0f : o[k] / l;
-                if (failed) y = __uint_as_float(0x7FC00000u);
-                store1(a.out, a.type, (int64_t)row * a.out_stride + (int64_t)head * D + lane + 64 * k, y);
+        const int i = __builtin_ctzll(__ballot(lines[wave][lane].end > at - base));
+        const Line& ln = lines[wave][i];
+        const KvSeq s = {__builtin_amdgcn_readfirstlane(ln.s.slot), __builtin_amdgcn_readfirstlane(ln.s.len),
+                         __builtin_amdgcn_readfirstlane(ln.s.row0), __builtin_amdgcn_readfirstlane(ln.s.n)};
+        const int tiles = __builtin_amdgcn_readfirstlane(ln.tiles), rows = s.n * a.G;
+        const uint32_t before = at - base - (__builtin_amdgcn_readfirstlane(ln.end) - (uint32_t)tiles * a.c.H);
+        const int kvh = before / tiles, p_begin = before - kvh * tiles, share = min((int)(to - at), tiles - p_begin);
+        at += share;
+        const Range g = range_of(a, s, 0, rows);
+        const int t_begin = max(0, p_begin - START), t_end = p_begin + share - START;
+        if (t_end < 0 || (t_end == 0 && g.tiles > 0)) continue;  // the next wave begins it
+        const int count = t_end - t_begin;  // (none where nothing is visible)
+        const int first = g.begin + t_begin;
+
+        const int r = min(col, rows - 1), head = kvh * a.G + r % a.G, row = s.row0 + r / a.G, pos = g.base + r / a.G;
+        const int whole_hi = a.causal ? min(s.len, g.base + 1) : s.len;
+        const int whole_lo = a.window ? max(0, g.base + s.n - a.window) : 0;
+        Carry<NR, DT> cy;
+        carry_init(cy);
+        attend_tiles<NR, DT, ND, EXT, true>(cy, a, s, kvh, row, head, col < rows, pos, first, 1, count, whole_lo, whole_hi);
+        cy.l = row_sum<NR>(cy.l);
+        if (count == g.tiles) {
+            const float f = failed ? __uint_as_float(0x7FC00000u) : cy.l == 0.0f ? 0.0f : cy.R / cy.l;
+            if (col < rows) put_out(cy, a, (int64_t)row * a.out_stride + (int64_t)head * D, gl, f);
+        } else {
+            const int slot = t_begin == 0;
+            const int p = (wave * 2 + slot) * a.rows_cap + col;
+            if (a.group == 1) {
+                const int64_t q = ((int64_t)w * 2 + slot) * a.rows_cap + col;
+                if (col < rows) {
+                    put_sums(cy, a.part_o + q * D, gl, cy.R);
+                    if (gl == 0) reinterpret_cast<float2*>(a.part_ml)[q] = make_float2(cy.m, cy.l);
+                }
+                continue;
             }
+            if (col < rows) {
+                put_sums(cy, sums + (size_t)p * D, gl, cy.R);
+                if (gl == 0) stats[p] = make_float2(cy.m, cy.l);
+            }
+            if (lane == 0) parts[wave][slot] = Part{rows, s.row0, kvh, t_end == g.tiles};
+        }
+    }
+    if (a.group == 1) return;
+    __syncthreads();
+    // the workgroup's parts: each one that does not continue a part of the wave before, with those that continue it
+    for (int f = 0; f < 8; ++f) {
+        const int fw = f >> 1, slot = f & 1;
+        const Part part = parts[fw][slot];
+        if (part.rows == 0 || (slot == 0 && fw > 0)) continue;
+        int last = fw;
+        bool ends = part.ends;
+        while (!ends && last + 1 < 4 && parts[last + 1][0].rows) ends = parts[++last][0].ends;
+        const bool whole = slot == 1 && ends;
+        for (int i = threadIdx.x; i < part.rows * D; i += 256) {
+            const int rr = i / D, d = i - rr * D;
+            float m = -__builtin_inff();
+            for (int u = fw; u <= last; ++u) m = fmaxf(m, stats[(u * 2 + (u == fw ? slot : 0)) * a.rows_cap + rr].x);
+            float o = 0.0f, l = 0.0f;
+            for (int u = fw; u <= last; ++u) {
+                const int p = (u * 2 + (u == fw ? slot : 0)) * a.rows_cap + rr;
+                const float2 ml = stats[p];
+                const float e = ml.x == m ? 1.0f : __builtin_amdgcn_exp2f(ml.x - m);
+                l = __builtin_fmaf(e, ml.y, l);
+                o = __builtin_fmaf(e, sums[(size_t)p * D + d], o);
+            }
+            if (whole) {
+                float y = l == 0.0f ? 0.0f : o / l;
+                if (failed) y = __uint_as_float(0x7FC00000u);
+                store1(a.out, a.type, (int64_t)(part.row0 + rr / a.G) * a.out_stride + (int64_t)(part.kvh * a.G + rr % a.G) * D + d, y);
+            } else {
+                const int64_t p = ((int64_t)(blockIdx.x * 4 + fw) * 2 + slot) * a.rows_cap + rr;
+                a.part_o[p * D + d] = o;
+                if (d == 0) reinterpret_cast<float2*>(a.part_ml)[p] = make_float2(m, l);
+            }
+        }
     }
 }
 
-template <int DT>
-void launch_dt(const AttendArgs& a, hipStream_t st) {
+// blockIdx.x = sequence * H + kv head; the rows over blockIdx.y
+__global__ __launch_bounds__(256) void k_attend_stream_join(const AttendArgs a) {
+    const int seq = blockIdx.x / a.c.H, kvh = blockIdx.x % a.c.H;
+    const int failed = *a.c.status;
+    uint32_t total = 0, begin = 0;
+    KvSeq s = {0, 0, 0, 0};
+    int tiles = 0;
+    for (int c = 0; c < a.b.n_seqs; c += 64) {
+        const Line n = line_of(a, c);
+        if (c == (seq & ~63)) {
+            const int i = seq & 63;
+            s = KvSeq{lane_of(n.s.slot, i), lane_of(n.s.len, i), lane_of(n.s.row0, i), lane_of(n.s.n, i)};
+            tiles = lane_of(n.tiles, i);
+            begin = total + lane_of(n.end, i) - (uint32_t)tiles * (a.c.H - kvh);
+        }
+        total += lane_of(n.end, 63);
+    }
+    const int rows = s.n * a.G, per = per_wave(a, total);
+    if (tiles <= START) return;
+    const int w0 = (begin + START) / per, b0 = w0 / a.group, b1 = (int)((begin + tiles - 1) / per) / a.group;
+    if (b0 == b1) return;
+    auto part = [&](int i) { return i == 0 ? (int64_t)w0 * 2 + 1 : (int64_t)(b0 + i) * a.group * 2; };
+    auto place = [&](int r) { return (int64_t)(s.row0 + r / a.G) * a.out_stride + (int64_t)(kvh * a.G + r % a.G) * a.c.D; };
+    if (b1 - b0 < 2 * FLIGHT) {  // few partials: a wave for each row
+        for (int r = blockIdx.y * 4 + (threadIdx.x >> 6); r < rows; r += gridDim.y * 4) join_row<1>(a, b1 - b0 + 1, r, place(r), failed, part);
+        return;
+    }
+    for (int r = blockIdx.y; r < rows; r += gridDim.y) {
+        join_row<4>(a, b1 - b0 + 1, r, place(r), failed, part);
+        __syncthreads();
+    }
+}
+
+template <int NR, int DT>
+void launch_form(const AttendArgs& a, hipStream_t st) {
+    const bool ext = a.cap > 0.0f || a.alibi, wide = a.type == JX_TYPE_F32;
+    if (a.waves) {
+        auto k = wide ? (ext ? k_attend_stream<NR, DT, 3, true> : k_attend_stream<NR, DT, 3, false>)
+                      : (ext ? k_attend_stream<NR, DT, 2, true> : k_attend_stream<NR, DT, 2, false>);
+        const size_t lds = a.group == 1 ? 0 : stream_lds(a.rows_cap, a.c.D);
+        if (lds > 65536 - 8192)
+            (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        hipLaunchKernelGGL(k, dim3(a.waves / 4), dim3(256), lds, st, a);
+        return;
+    }
     const size_t lds = sizeof(float) * (size_t)waves_of(DT) * a.rows_cap * (a.c.D + 2);
     const dim3 grid((unsigned)((int64_t)a.b.n_seqs * a.splits * a.row_tiles * a.c.H));
-    const bool ext = a.cap > 0.0f || a.alibi, wide = a.type == JX_TYPE_F32;
-    auto k = wide ? (ext ? k_attend<DT, 3, true> : k_attend<DT, 3, false>) : (ext ? k_attend<DT, 2, true> : k_attend<DT, 2, false>);
+    auto k = wide ? (ext ? k_attend<NR, DT, 3, true> : k_attend<NR, DT, 3, false>) : (ext ? k_attend<NR, DT, 2, true> : k_attend<NR, DT, 2, false>);
     if (lds > 65536)
         (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     hipLaunchKernelGGL(k, grid, dim3(64 * waves_of(DT)), lds, st, a);
+    if (a.splits > 1)
+        hipLaunchKernelGGL(k_attend_join<NR>, dim3((unsigned)((int64_t)a.b.n_seqs * a.row_tiles * a.c.H), a.rows_cap), dim3(256), 0, st, a);
+}
+template <int DT>
+void launch_dt(const AttendArgs& a, hipStream_t st) {
+    if (a.rows_cap <= 16)
+        launch_form<16, DT>(a, st);
+    else
+        launch_form<32, DT>(a, st);
 }
 
 }  // namespace
@@ -454,16 +931,35 @@ void launch_dt(const AttendArgs& a, hipStream_t st) {
 AttendPlan attend_plan(const jx_kv_cache& c, const jx_kv_batch& b, const jx_attention& t) {
     AttendPlan p;
     const int64_t most = (int64_t)c.max_pages * c.page_tokens;
-    const int G = t.n_heads / c.n_kv_heads;
+    const int G = t.n_heads / c.n_kv_heads, W = waves_of(c.head_dim / 32);
     p.row_tiles = (int)(((int64_t)b.max_rows * G + 31) / 32);
+    p.rows_cap = (int)std::min<int64_t>(32, (int64_t)b.max_rows * G);
     int64_t len = b.max_len > 0 ? std::min<int64_t>(b.max_len, most) : most;
     if (t.window > 0 && t.causal) len = std::min<int64_t>(len, (int64_t)t.window + b.max_rows + KV_BLOCK);
     const int64_t tiles = std::max<int64_t>(1, (len + KV_BLOCK - 1) / KV_BLOCK);
-    // about two workgroups for each of the 256 CUs, of at least two tiles per wave
     const int64_t items = (int64_t)b.n_seqs * p.row_tiles * c.n_kv_heads;
-    int64_t splits = std::max<int64_t>(1, std::min<int64_t>(512 / std::max<int64_t>(1, items), tiles / (2 * waves_of(c.head_dim / 32))));
+    p.splits = 1;
+    p.chunk = (int)tiles;
+    p.waves = 0;
+    p.group = 1;
+    p.partials = 0;
+    if (p.row_tiles == 1 && !(items <= 256 && tiles <= 4 * W) &&
+        (int64_t)b.n_seqs * c.n_kv_heads * ((most + KV_BLOCK - 1) / KV_BLOCK) < INT32_MAX) {
+        // as many waves as are resident at once: registers, and 160 KB of LDS less the workgroup's fixed 7
+        const size_t lds = stream_lds(p.rows_cap, c.head_dim);
+        // few sequences and heads have many parts each: 8 of them 57 us with a group's parts joined and 58 without, 64 (draft
+        // tokens, 10 rows of 256 dimensions) 32 and 33; 272 and 512 of them 22 and 21, 60 and 58
+        p.group = items <= 128 && lds <= 150 * 1024 ? 4 : 1;
+        const int by_registers = stream_occupancy(p.rows_cap <= 16 ? 16 : 32, c.head_dim / 32);
+        p.waves = 256 * 4 * (p.group == 4 && lds > 72 * 1024 ? 1 : by_registers);
+        p.partials = 2 * (int64_t)p.waves;
+        return p;
+    }
+    // about two workgroups for each of the 256 CUs, of at least two tiles per wave
+    const int64_t splits = std::max<int64_t>(1, std::min<int64_t>(512 / std::max<int64_t>(1, items), tiles / (2 * W)));
     p.chunk = (int)((tiles + splits - 1) / splits);
     p.splits = (int)((tiles + p.chunk - 1) / p.chunk);
+    if (p.splits > 1) p.partials = items * p.splits;
     return p;
 }
 
@@ -478,8 +974,10 @@ void launch_attend(const AttendArgs& a, hipStream_t st) {
         case 7: launch_dt<7>(a, st); break;
         default: launch_dt<8>(a, st); break;
     }
-    if (a.splits > 1)
-        hipLaunchKernelGGL(k_attend_join, dim3((unsigned)((int64_t)a.b.n_seqs * a.row_tiles * a.c.H)), dim3(256), 0, st, a);
+    if (a.waves)
+        // few sequences and heads: a workgroup per row (many partials each); many: one for all rows
+        hipLaunchKernelGGL(k_attend_stream_join, dim3((unsigned)((int64_t)a.b.n_seqs * a.c.H), (int64_t)a.b.n_seqs * a.c.H <= 128 ? a.rows_cap : 1),
+                           dim3(256), 0, st, a);
 }
 
 }  // namespace jx

@@ -51,7 +51,7 @@ __device__ __forceinline__ KvSeq kv_seq(const KvView& c, const KvRows& b, int i)
                     (int64_t)s.len <= (int64_t)c.max_pages * c.page_tokens;
     s.row0 = r0;
     s.n = ok ? r1 - r0 : 0;
-    if (!ok && threadIdx.x == 0) atomicOr(c.status, JX_KV_BAD_ARG);
+    if (!ok) atomicOr(c.status, JX_KV_BAD_ARG);
     return s;
 }
 
@@ -62,8 +62,8 @@ struct AttendArgs {
     void* out;
     int64_t q_stride, out_stride;
     const float* alibi;
-    float* part_o;   // [n_rows][n_heads][splits][D] sums of weights times values
-    float* part_ml;  // [n_rows][n_heads][splits][2] the running maximum and the sum of weights
+    float* part_o;   // [partials][rows_cap][D] sums of weights times values
+    float* part_ml;  // [partials][rows_cap][2] the running maximum and the sum of weights
     int type, heads, G;
     float scale2;    // scale * log2(e)
     float cap;       // 0: none (natural units)
@@ -71,6 +71,8 @@ struct AttendArgs {
     int window, causal;
     int chunk;       // tiles of 32 tokens that a workgroup takes at most, unless that makes more than `splits` of a sequence
     int splits;
+    int waves;       // k_attend_stream: waves of the launch
+    int group;       //   waves whose parts become one partial
     int row_tiles;   // of the sequence with the most rows
     int rows_cap;    // rows of a row tile at most: min(tile, max_rows * G)
     bool q_vec, out_vec;  // 16-byte aligned rows
@@ -78,7 +80,9 @@ struct AttendArgs {
 
 // How many splits the launch for this batch takes, and its chunk; the workspace is sized by it.
 struct AttendPlan {
-    int splits, chunk, row_tiles;
+    int splits, chunk, row_tiles, rows_cap;
+    int waves, group;  // waves not 0: k_attend_stream
+    int64_t partials;  // of the workspace, each rows_cap rows of D + 2 floats
 };
 AttendPlan attend_plan(const jx_kv_cache& c, const jx_kv_batch& b, const jx_attention& a);
 void launch_attend(const AttendArgs& a, hipStream_t st);

@@ -683,8 +683,8 @@ int check_attention(const jx_kv_cache* c, const jx_kv_batch* b, const jx_attenti
     return JX_OK;
 }
 
-size_t workspace(const jx_kv_cache* c, const jx_kv_batch* b, const jx_attention* t, const AttendPlan& p) {
-    return p.splits > 1 ? (size_t)b->n_rows * t->n_heads * p.splits * (c->head_dim + 2) * sizeof(float) : 0;
+size_t workspace(const jx_kv_cache* c, const AttendPlan& p) {
+    return (size_t)p.partials * p.rows_cap * (c->head_dim + 2) * sizeof(float);
 }
 
 }  // namespace
@@ -761,7 +761,7 @@ int jx_kv_append(const jx_kv_cache* c, const jx_kv_batch* b, int32_t layer, int3
 
 size_t jx_kv_attention_workspace(const jx_kv_cache* c, const jx_kv_batch* b, const jx_attention* t) {
     if (check_attention(c, b, t) != JX_OK || b->n_seqs == 0 || b->max_rows == 0) return 0;
-    return workspace(c, b, t, attend_plan(*c, *b, *t));
+    return workspace(c, attend_plan(*c, *b, *t));
 }
 
 int jx_kv_attention(const jx_kv_cache* c, const jx_kv_batch* b, const jx_attention* t, int32_t layer, const void* q, void* out,
@@ -775,7 +775,7 @@ int jx_kv_attention(const jx_kv_cache* c, const jx_kv_batch* b, const jx_attenti
     const size_t size = type_size(t->type);
     REFUSE(!aligned(q, size) || !aligned(out, size), JX_ERR_INVALID, "q or out is not aligned");
     const AttendPlan p = attend_plan(*c, *b, *t);
-    const size_t need = workspace(c, b, t, p);
+    const size_t need = workspace(c, p);
     REFUSE(need && (!ws || ws_bytes < need), JX_ERR_INVALID, "the workspace is smaller than jx_kv_attention_workspace()");
     REFUSE(need && !aligned(ws, 16), JX_ERR_INVALID, "the workspace is not 16-byte aligned");
     REFUSE((int64_t)b->n_seqs * p.splits * p.row_tiles * c->n_kv_heads > INT32_MAX, JX_ERR_UNSUPPORTED,
@@ -792,7 +792,7 @@ int jx_kv_attention(const jx_kv_cache* c, const jx_kv_batch* b, const jx_attenti
     a.out_stride = t->out_stride ? t->out_stride : width;
     a.alibi = t->alibi;
     a.part_o = static_cast<float*>(ws);
-    a.part_ml = a.part_o + (size_t)b->n_rows * t->n_heads * p.splits * c->head_dim;
+    a.part_ml = a.part_o + (size_t)p.partials * p.rows_cap * c->head_dim;
     a.type = t->type;
     a.heads = t->n_heads;
     a.G = t->n_heads / c->n_kv_heads;
@@ -803,8 +803,10 @@ int jx_kv_attention(const jx_kv_cache* c, const jx_kv_batch* b, const jx_attenti
     a.causal = t->causal;
     a.chunk = p.chunk;
     a.splits = p.splits;
+    a.waves = p.waves;
+    a.group = p.group;
     a.row_tiles = p.row_tiles;
-    a.rows_cap = (int)std::min<int64_t>(32, (int64_t)b->max_rows * a.G);
+    a.rows_cap = p.rows_cap;
     a.q_vec = aligned(q, 16) && a.q_stride * size % 16 == 0;
     a.out_vec = aligned(out, 16) && a.out_stride * size % 16 == 0;
     launch_attend(a, reinterpret_cast<hipStream_t>(stream));

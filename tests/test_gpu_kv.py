@@ -484,6 +484,18 @@ def test_attend_long(D, H, G, dtype):
     near(*p.attend([0, 1], [1, 1], H * G, dtype, window=5000))
 
 
+@pytest.mark.parametrize("D", [32, 64, 96, 128, 160, 192, 224, 256])
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_attend_uneven_batches(D, dtype):
+    """Few rows over sequences of very different lengths, 1 to 32 rows times heads, more sequences than a wave has lanes."""
+    for G, rows, lengths in ((1, 1, (1, 1500, 0, 37, 2300, 64)), (5, 3, (40, 1100, 2000, 7)), (16, 1, (1700, 3)), (17, 1, (1300, 90)),
+                             (4, 8, (8, 1200, 600)), (2, 1, tuple(int(x) for x in np.random.default_rng(D).integers(0, 300, 70)) + (1200,))):
+        p = filled(D=D, H=2, P=64, lengths=lengths, pages=260, seed=D + G, rotate=False)
+        say(f"uneven D={D} {dtype} G={G} rows={rows} sequences={len(lengths)}")
+        slots = list(range(len(lengths)))[::-1]
+        near(*p.attend(slots, [min(rows, lengths[s]) for s in slots], 2 * G, dtype, sharp=2.0, strided=G == 5))
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_attend_scales_apart(dtype):
     """Blocks whose scales lie far apart, zero blocks among them, in every order: weights stay in range."""
