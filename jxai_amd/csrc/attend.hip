@@ -201,7 +201,7 @@ __device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, ui
 //   u = rint(v * TOP / amax) + 64 (1 + 128): added to 1.5 2^23 by the multiply-add that forms it, u is in the low mantissa bits;
 //   its groups of 7 bits are the lower digits + 64, what is above them the top digit.
 template <int NR, int DT, int ND>
-__device__ __forceinline__ void digits(const Raw<NR, DT>& v, Digits<NR, DT, ND>& qd, float& qs) {
+__device__ __forceinline__ void digits(const Raw<NR, DT>& v, bool flip, Digits<NR, DT, ND>& qd, float& qs) {
     typedef Form<NR, DT> F;
     constexpr float TOP = ND == 2 ? 127.0f * 128.0f : 127.0f * 16384.0f;
     constexpr float MAGIC = 12582912.0f + (ND == 2 ? 64.0f : 64.0f + 64.0f * 128.0f);
@@ -216,7 +216,7 @@ __device__ __forceinline__ void digits(const Raw<NR, DT>& v, Digits<NR, DT, ND>&
     // rows below 2^-100 count as zero: TOP / amax stays finite
     const bool zero = top < 0x0D800000u;
     const float amax = __uint_as_float(top);
-    const float inv = finite && !zero ? TOP / amax : 0.0f;
+    const float inv = finite && !zero ? (flip ? -TOP : TOP) / amax : 0.0f;
     qs = !finite ? __uint_as_float(0x7FC00000u) : zero ? 0.0f : amax / TOP;
 #pragma unroll
     for (int j = 0; j < F::STEPS; ++j)
@@ -284,33 +284,41 @@ __device__ __forceinline__ void scores(Scores<NR, DT, ND>& acc, const Digits<NR,
             for (int n = 0; n < ND; ++n) acc[n][t] = F::scores(kc[t][j], qd[n][j], acc[n][t]);
 }
 
-// The rest of the block, whose tokens begin at t0.  lo / hi: the lane's row sees tokens lo .. hi - 1 (masked: whether to look).
+// The weights of a lane's row and tokens as operand of the product with V, in the order of V's bytes; e: what their rounding
+// left (fp32: 22 bits in all).
+template <int NR, int ND>
+struct Weights {
+    h8 p[NR / 16], e[ND == 3 ? NR / 16 : 1];
+};
+
+// From S^T of a block whose tokens begin at t0.  lo / hi: the lane's row sees tokens lo .. hi - 1 (masked: whether to look).
 template <int NR, int DT, int ND, bool EXT>
-__device__ __forceinline__ void weigh(Carry<NR, DT>& s, const AttendArgs& a, const Scores<NR, DT, ND>& acc,
-                                      float qs, float slope, int pos, const v4i (&vc)[DT], float ks, float vs, int t0, int g, int lo,
-                                      int hi, bool masked) {
+__device__ __forceinline__ Weights<NR, ND> weights(Carry<NR, DT>& s, const AttendArgs& a, const Scores<NR, DT, ND>& acc, float qs, float slope,
+                                                   int pos, float ks, float vs, int t0, int g, int lo, int hi, bool masked) {
     typedef Form<NR, DT> F;
     constexpr int X = F::X, PER = X / F::ACCS;
     float x[X];
-    const float c = qs * ks * (EXT ? a.scale : a.scale2);
 #pragma unroll
     for (int i = 0; i < X; ++i) {
         const int t = i / PER, k = i % PER;
         // |acc| <= 127 * 127 * 256: two digits fit an int32
         if constexpr (ND == 2)
-            x[i] = (float)(acc[0][t][k] * 128 + acc[1][t][k]) * c;
+            x[i] = (float)(int)(((uint32_t)acc[0][t][k] << 7) + (uint32_t)acc[1][t][k]);
         else
-            x[i] = __builtin_fmaf((float)acc[0][t][k], 16384.0f, (float)(acc[1][t][k] * 128 + acc[2][t][k])) * c;
+            x[i] = __builtin_fmaf((float)acc[0][t][k], 16384.0f, (float)(int)(((uint32_t)acc[1][t][k] << 7) + (uint32_t)acc[2][t][k]));
     }
+    // x * c is the exponent of 2.  (c is kept above 0, so that a masked -inf stays what it is; the sign of the softmax scale is in q.)
+    float c = qs * ks * (EXT ? a.scale : a.scale2);
+    c = c < 1e-30f ? 1e-30f : c;
     if constexpr (EXT) {
-        if (a.cap > 0.0f) {
-            const float inv = 1.0f / a.cap;
+        const float inv = a.cap > 0.0f ? 1.0f / a.cap : 0.0f, d0 = (float)(t0 + 4 * g - pos);
 #pragma unroll
-            for (int i = 0; i < X; ++i) x[i] = a.cap * tanh_fast(x[i] * inv);
+        for (int i = 0; i < X; ++i) {
+            x[i] *= c;
+            if (a.cap > 0.0f) x[i] = a.cap * tanh_fast(x[i] * inv);
+            x[i] = __builtin_fmaf(slope, d0 + (float)F::token(i), x[i]);
         }
-        const float d0 = (float)(t0 + 4 * g - pos);
-#pragma unroll
-        for (int i = 0; i < X; ++i) x[i] = __builtin_fmaf(slope, d0 + (float)F::token(i), x[i]) * LOG2E;
+        c = LOG2E;
     }
     const int l0 = lo - t0 - 4 * g, h0 = hi - t0 - 4 * g;
     if (masked) {
@@ -320,7 +328,7 @@ __device__ __forceinline__ void weigh(Carry<NR, DT>& s, const AttendArgs& a, con
     float top = x[0];
 #pragma unroll
     for (int i = 1; i < X; ++i) top = fmaxf(top, x[i]);
-    top = row_max<NR>(top);
+    top = row_max<NR>(top) * c;
     if (__any(top > s.m + LAG)) {
         const float m = fmaxf(s.m, top);
         const float f = m == s.m ? 1.0f : __builtin_amdgcn_exp2f(s.m - m);
@@ -332,68 +340,73 @@ __device__ __forceinline__ void weigh(Carry<NR, DT>& s, const AttendArgs& a, con
         carry_scale(s, s.R / vs);
         s.R = vs;
     }
-    // a block of zeros has scale 0; NaN marks a block that reads as NaN
+    // V's scale goes into the exponent and out of the sum again where it is not too small beside R; otherwise (a block of
+    // zeros has scale 0, and NaN marks one that reads as NaN) into the weights behind the sum.
     const float vr = vs == s.R && vs > 0.0f ? 1.0f : vs == 0.0f ? 0.0f : vs / s.R;
-    const float ref = s.m == -__builtin_inff() ? (float)-OFF : s.m - (float)OFF;
+    const bool near = vr >= 0x1p-20f;
+    const float ref = (s.m == -__builtin_inff() ? 0.0f : s.m) - (float)OFF - (near ? __builtin_amdgcn_logf(vr) : 0.0f);
     float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < X; ++i) {
-        const float p = __builtin_amdgcn_exp2f(x[i] - ref);
-        sum += p;
-        x[i] = p * vr;
+        x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], c, -ref));
+        sum += x[i];
     }
-    if (masked) {  // nothing of a NaN scale reaches a row that does not see the block
+    if (near) {
+        s.l = __builtin_fmaf(sum, __builtin_amdgcn_rcpf(vr), s.l);
+    } else {
+        s.l += sum;
 #pragma unroll
-        for (int i = 0; i < X; ++i) x[i] = F::token(i) >= l0 && F::token(i) < h0 ? x[i] : 0.0f;
+        for (int i = 0; i < X; ++i) x[i] *= vr;
+        if (masked) {  // nothing of a NaN scale reaches a row that does not see the block
+#pragma unroll
+            for (int i = 0; i < X; ++i) x[i] = F::token(i) >= l0 && F::token(i) < h0 ? x[i] : 0.0f;
+        }
     }
-    s.l += sum;
-    if constexpr (NR == 32) {
-        // token 8 a + 4 g + b is register 4 a + b here and byte 8 (a & 1) + 4 (a >> 1) + b of V
-        h8 p0, p1, e0, e1;
+    // 32 rows: token 8 a + 4 g + b is register 4 a + b here and byte 8 (a & 1) + 4 (a >> 1) + b of V.  16 rows: in order
+    Weights<NR, ND> w;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            p0[i] = (_Float16)x[i], p0[4 + i] = (_Float16)x[8 + i];
-            p1[i] = (_Float16)x[4 + i], p1[4 + i] = (_Float16)x[12 + i];
-        }
-        if constexpr (ND == 3) {  // the weights' remainders: 22 bits in all
+    for (int i = 0; i < X; ++i) {
+        const int o = NR == 32 ? (i >> 2) & 1 : 0, at = NR == 32 ? 4 * (i >> 3) + (i & 3) : i;
+        w.p[o][at] = (_Float16)x[i];
+        if constexpr (ND == 3) w.e[o][at] = (_Float16)(x[i] - (float)w.p[o][at]);
+    }
+    return w;
+}
+
+template <int NR>
+__device__ __forceinline__ auto value_mfma(h8 v, h8 p, typename Form<NR, 1>::Out o) {
+    if constexpr (NR == 32)
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p, o, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p, o, 0, 0, 0);
+}
+
+// Their product with V from its codes in registers
+template <int NR, int DT, int ND>
+__device__ __forceinline__ void add_values(Carry<NR, DT>& s, const Weights<NR, ND>& w, const v4i (&vc)[DT]) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                e0[i] = (_Float16)(x[i] - (float)p0[i]), e0[4 + i] = (_Float16)(x[8 + i] - (float)p0[4 + i]);
-                e1[i] = (_Float16)(x[4 + i] - (float)p1[i]), e1[4 + i] = (_Float16)(x[12 + i] - (float)p1[4 + i]);
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < DT; ++i) {
+    for (int i = 0; i < DT; ++i) {
+        if constexpr (NR == 32) {
             const h8 v0 = codes_to_half((uint32_t)vc[i][0], (uint32_t)vc[i][1]);
             const h8 v1 = codes_to_half((uint32_t)vc[i][2], (uint32_t)vc[i][3]);
-            s.o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v0, p0, s.o[i], 0, 0, 0);
-            s.o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v1, p1, s.o[i], 0, 0, 0);
+            s.o[i] = value_mfma<NR>(v0, w.p[0], s.o[i]);
+            s.o[i] = value_mfma<NR>(v1, w.p[1], s.o[i]);
             if constexpr (ND == 3) {
-                s.o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v0, e0, s.o[i], 0, 0, 0);
-                s.o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v1, e1, s.o[i], 0, 0, 0);
+                s.o[i] = value_mfma<NR>(v0, w.e[0], s.o[i]);
+                s.o[i] = value_mfma<NR>(v1, w.e[1], s.o[i]);
             }
-        }
-    } else {
-        // registers 0 .. 3 are tokens 4 g + b, 4 .. 7 tokens 16 + 4 g + b: of a piece (h, d) of V the eight bytes from
-        // 8 (g >> 1) on, h = g & 1.  The lane loaded all 16 bytes of piece h of dimension 32 i + 16 (g >> 1) + col: the
-        // halves of the wave exchange what belongs to the other's 16 dimensions.
-        h8 p, e;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) p[i] = (_Float16)x[i];
-        if constexpr (ND == 3) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) e[i] = (_Float16)(x[i] - (float)p[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < DT; ++i) {
+        } else {
+            // registers 0 .. 3 are tokens 4 g + b, 4 .. 7 tokens 16 + 4 g + b: of a piece (h, d) of V the eight bytes from
+            // 8 (g >> 1) on, h = g & 1.  The lane loaded all 16 bytes of piece h of dimension 32 i + 16 (g >> 1) + col: the
+            // halves of the wave exchange what belongs to the other's 16 dimensions.
             const auto r0 = __builtin_amdgcn_permlane32_swap((uint32_t)vc[i][0], (uint32_t)vc[i][2], false, false);
             const auto r1 = __builtin_amdgcn_permlane32_swap((uint32_t)vc[i][1], (uint32_t)vc[i][3], false, false);
             const h8 v0 = codes_to_half(r0[0], r1[0]), v1 = codes_to_half(r0[1], r1[1]);
-            s.o[2 * i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, p, s.o[2 * i], 0, 0, 0);
-            s.o[2 * i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, p, s.o[2 * i + 1], 0, 0, 0);
+            s.o[2 * i] = value_mfma<NR>(v0, w.p[0], s.o[2 * i]);
+            s.o[2 * i + 1] = value_mfma<NR>(v1, w.p[0], s.o[2 * i + 1]);
             if constexpr (ND == 3) {
-                s.o[2 * i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, e, s.o[2 * i], 0, 0, 0);
-                s.o[2 * i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, e, s.o[2 * i + 1], 0, 0, 0);
+                s.o[2 * i] = value_mfma<NR>(v0, w.e[0], s.o[2 * i]);
+                s.o[2 * i + 1] = value_mfma<NR>(v1, w.e[0], s.o[2 * i + 1]);
             }
         }
     }
@@ -476,7 +489,7 @@ __device__ __forceinline__ void attend_tiles(Carry<NR, DT>& cy, const AttendArgs
     }
     Digits<NR, DT, ND> qd;
     float qs;
-    digits<NR, DT, ND>(raw, qd, qs);
+    digits<NR, DT, ND>(raw, a.flip, qd, qs);
     for (int b0 = 0; b0 < count; b0 += 64) {
         const int n = min(64, count - b0);
         if (b0) {
@@ -490,8 +503,9 @@ __device__ __forceinline__ void attend_tiles(Carry<NR, DT>& cy, const AttendArgs
             scores<NR, DT, ND>(acc, qd, k);
             if (i + 1 < n) fetch_k(i + 1);
             const int t0 = (first + (b0 + i) * step) * KV_BLOCK;
-            weigh<NR, DT, ND, EXT>(cy, a, acc, qs, slope, pos, v, lane_of(bl.ks, i), lane_of(bl.vs, i), t0, g, lo, hi,
-                                   t0 < whole_lo || t0 + KV_BLOCK > whole_hi);
+            const auto w = weights<NR, DT, ND, EXT>(cy, a, acc, qs, slope, pos, lane_of(bl.ks, i), lane_of(bl.vs, i), t0, g, lo, hi,
+                                                    t0 < whole_lo || t0 + KV_BLOCK > whole_hi);
+            add_values<NR, DT, ND>(cy, w, v);
             if (i + 1 < n) fetch_v(i + 1);
         }
     }
@@ -544,69 +558,198 @@ __device__ __forceinline__ Range range_of(const AttendArgs& a, const KvSeq& s, i
 // Waves of a workgroup: wide heads need more than 256 registers, and LDS for the join.
 __host__ __device__ constexpr int waves_of(int dt) { return dt <= 4 ? 8 : 4; }
 
-// blockIdx.x = ((sequence * splits + split) * row_tiles + row tile) * H + kv head.  The waves of a workgroup take the tiles of
-// its split in turn and join in LDS.
+// Up to 32 rows over a short sequence: a workgroup for each sequence and kv head (blockIdx.x = sequence * H + kv head), whose waves
+// take its tiles in turn and join in LDS.  One launch: the form for latency.
 template <int NR, int DT, int ND, bool EXT>
 __global__ __launch_bounds__(64 * waves_of(DT)) void k_attend(const AttendArgs a) {
     extern __shared__ float lds[];
-    const int W = blockDim.x >> 6, wave = threadIdx.x >> 6, lane = threadIdx.x & 63, gl = lane / NR, col = lane % NR;
+    constexpr int W = waves_of(DT);
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, gl = lane / NR, col = lane % NR, D = a.c.D;
+    const int kvh = blockIdx.x % a.c.H, seq = blockIdx.x / a.c.H;
+    const int failed = *a.c.status;
+    const KvSeq s = kv_seq(a.c, a.b, seq);
+    const int rows = s.n * a.G;
+    if (rows == 0) return;
+    const Range g = range_of(a, s, 0, rows);
+    const int r = min(col, rows - 1), head = kvh * a.G + r % a.G, row = s.row0 + r / a.G, pos = g.base + r / a.G;
+    // tiles that every row sees whole need no mask: hi of the first row, lo of the last
+    const int whole_hi = a.causal ? min(s.len, g.base + 1) : s.len, whole_lo = a.window ? max(0, g.base + s.n - a.window) : 0;
+    Carry<NR, DT> cy;
+    carry_init(cy);
+    attend_tiles<NR, DT, ND, EXT, false>(cy, a, s, kvh, row, head, col < rows, pos, g.begin + wave, W, (g.tiles - wave + W - 1) / W,
+                                         whole_lo, whole_hi);
+
+    // the waves' sums: [W][rows_cap][D], then [W][rows_cap] of the maximum and the sum of weights
+    float* so = lds;
+    float2* sm = reinterpret_cast<float2*>(lds + (size_t)W * a.rows_cap * D);
+    cy.l = row_sum<NR>(cy.l);
+    if (col < rows) {
+        put_sums(cy, so + ((size_t)wave * a.rows_cap + col) * D, gl, cy.R);
+        if (gl == 0) sm[wave * a.rows_cap + col] = make_float2(cy.m, cy.l);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < rows * D; i += 64 * W) {
+        const int rr = i / D, d = i - rr * D;
+        float m = -__builtin_inff(), o = 0.0f, l = 0.0f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) m = fmaxf(m, sm[w * a.rows_cap + rr].x);
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const float2 ml = sm[w * a.rows_cap + rr];
+            const float f = ml.x == m ? 1.0f : __builtin_amdgcn_exp2f(ml.x - m);
+            l = __builtin_fmaf(f, ml.y, l);
+            o = __builtin_fmaf(f, so[((size_t)w * a.rows_cap + rr) * D + d], o);
+        }
+        float y = l == 0.0f ? 0.0f : o / l;
+        if (failed) y = __uint_as_float(0x7FC00000u);
+        store1(a.out, a.type, (int64_t)(s.row0 + rr / a.G) * a.out_stride + (int64_t)(kvh * a.G + rr % a.G) * D + d, y);
+    }
+}
+
+// ---------------------------------------------------------------- many rows: K and V through LDS
+
+constexpr int rows_waves(int dt) { return dt <= 4 ? 8 : 4; }  // (more than 128 dimensions: one wave per SIMD)
+constexpr int STAGE = 2;                                      // blocks of 32 tokens in LDS at a time
+
+// 32 rows per wave, 8 (4) waves against the same blocks.  A stage of two blocks goes through registers into one of two LDS
+// buffers: K's codes as they are, V's as fp16 in the order that the products read (converted once for all waves).  Both are
+// read and written 16 bytes per lane in a row.  While a stage is worked on, the next one is written and the one behind
+// it loaded; one barrier per stage.
+// blockIdx.x = ((sequence * splits + split) * row_tiles + row tile from the last) * H + kv head: the longest rows of a
+// causal prompt first, and the row tiles of 8 kv heads each on an XCD of their own, whose L2 keeps the head's K and V.
+template <int DT, int ND, bool EXT>
+__global__ __launch_bounds__(64 * rows_waves(DT), DT <= 4 ? 2 : 1) void k_attend_rows(const AttendArgs a) {
+    constexpr int W = rows_waves(DT), KB = 1024 * DT, VB = 2048 * DT, BUF = STAGE * (KB + VB);
+    constexpr int LOADS = (2 * STAGE * DT + W - 1) / W;  // of 1 KB per wave and stage
+    extern __shared__ uint4 lds4[];
+    __shared__ Blocks ring[128];
+    uint8_t* lds = reinterpret_cast<uint8_t*>(lds4);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, gl = lane >> 5, col = lane & 31;
     int item = blockIdx.x;
     const int kvh = item % a.c.H;
     item /= a.c.H;
-    const int rt = item % a.row_tiles;
+    const int rt = a.row_tiles - 1 - item % a.row_tiles;
     item /= a.row_tiles;
     const int split = item % a.splits, seq = item / a.splits;
     const int failed = *a.c.status;
     const KvSeq s = kv_seq(a.c, a.b, seq);
-    const int rows = s.n * a.G, r0 = rt * NR;
+    const int rows = s.n * a.G, r0 = rt * a.tile_rows;
     if (r0 >= rows) return;
-    const int nr = min(NR, rows - r0);
+    const int nr = min(a.tile_rows, rows - r0);
     const Range g = range_of(a, s, r0, nr);
     if (split >= g.n) return;
-    const int r = r0 + min(col, nr - 1), head = kvh * a.G + r % a.G, row = s.row0 + r / a.G, pos = g.base + r / a.G;
-    // tiles that every row sees whole need no mask: hi of the first row, lo of the last
-    const int p0 = g.base + r0 / a.G, p1 = g.base + (r0 + nr - 1) / a.G;
+    // the wave's rows
+    const int w0 = r0 + 32 * wave, wn = min(32, r0 + nr - w0);  // (wn <= 0: a wave without rows only moves the blocks)
+    const int r = min(w0 + col, rows - 1), head = kvh * a.G + r % a.G, row = s.row0 + r / a.G, pos = g.base + r / a.G;
+    const int hi = a.causal ? min(s.len, pos + 1) : s.len, lo = a.window ? max(0, pos - a.window + 1) : 0;
+    const int p0 = g.base + min(w0, rows - 1) / a.G, p1 = g.base + min(w0 + 31, rows - 1) / a.G;
+    // tokens that some row of the wave sees, and that every row sees
+    const int some_hi = wn <= 0 ? 0 : a.causal ? min(s.len, p1 + 1) : s.len, some_lo = a.window ? max(0, p0 - a.window + 1) : 0;
     const int whole_hi = a.causal ? min(s.len, p0 + 1) : s.len, whole_lo = a.window ? max(0, p1 - a.window + 1) : 0;
-    Carry<NR, DT> cy;
-    carry_init(cy);
-    const int first = g.begin + split * g.per + wave, end = g.begin + min(g.tiles, (split + 1) * g.per);
-    attend_tiles<NR, DT, ND, EXT, false>(cy, a, s, kvh, row, head, col < nr, pos, first, W, first < end ? (end - first + W - 1) / W : 0,
-                                         whole_lo, whole_hi);
 
-    // the waves' sums: [W][rows_cap][D], then [W][rows_cap][2] with the maximum and the sum of weights
-    float* so = lds;
-    float* sm = lds + (size_t)W * a.rows_cap * a.c.D;
-    cy.l = row_sum<NR>(cy.l);
-    if (col < nr) {
-        put_sums(cy, so + ((size_t)wave * a.rows_cap + col) * a.c.D, gl, cy.R);
-        if (gl == 0) {
-            sm[(wave * a.rows_cap + col) * 2] = cy.m;
-            sm[(wave * a.rows_cap + col) * 2 + 1] = cy.l;
+    Carry<32, DT> cy;
+    carry_init(cy);
+    const int first = g.begin + split * g.per, count = min(g.tiles, (split + 1) * g.per) - split * g.per;
+    // load u = wave + i * W of a stage: K of its blocks, then V, a kilobyte each
+    uint4 in[LOADS];
+    auto fetch = [&](int t, auto block_of) {  // the stage from tile t on
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const int u = wave + i * W;
+            if (u >= 2 * STAGE * DT) break;
+            const int which = u >= STAGE * DT, v = u - which * STAGE * DT;
+            const int block = block_of(min(t + v / DT, count - 1), which);
+            in[i] = ld16(a.c.codes + (int64_t)block * KB + (v % DT) * 1024 + lane * 16);
         }
+    };
+    auto put = [&](int buf) {
+        uint8_t* to = lds + buf * BUF;
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const int u = wave + i * W;
+            if (u >= 2 * STAGE * DT) break;
+            const int which = u >= STAGE * DT, v = u - which * STAGE * DT, b = v / DT, kb = v % DT;
+            if (!which) {
+                *reinterpret_cast<uint4*>(to + b * (KB + VB) + kb * 1024 + lane * 16) = in[i];
+            } else {  // the lane's 16 bytes are piece (h, d): tokens of the first and of the second product
+                const int piece = kb * 64 + lane, h = piece / (32 * DT), d = piece % (32 * DT);
+                h8* o = reinterpret_cast<h8*>(to + b * (KB + VB) + KB) + (d >> 5) * 128 + h * 32 + (d & 31);
+                o[0] = codes_to_half(in[i].x, in[i].y);
+                o[64] = codes_to_half(in[i].z, in[i].w);
+            }
+        }
+    };
+    // blocks and scales of 128 tiles around the current one: wave 0 looks the next 64 up, a step per stage
+    auto keep = [&](int t, const Blocks& b) { ring[(t + lane) & 127] = b; };
+    auto ring_block = [&](int t, int which) { return __builtin_amdgcn_readfirstlane(which ? ring[t & 127].v : ring[t & 127].k); };
+    auto look = [&](int t) { return page_of(a, s.slot, first + t + lane, t + lane < count); };
+    auto find = [&](int t, int page) { return blocks_of(a, kvh, page, first + t + lane, t + lane < count); };
+
+    Digits<32, DT, ND> qd;
+    float qs, slope = 0.0f;
+    int page = look(0);
+    Blocks bl;
+    {
+        Raw<32, DT> raw;
+        load_q<32, DT>(a, row, head, gl, w0 + col < r0 + nr, raw);
+        if (EXT && a.alibi) slope = a.alibi[head];
+        bl = find(0, page);
+        if (count > 0) fetch(0, [&](int t, int which) { return which ? lane_of(bl.v, t) : lane_of(bl.k, t); });
+        digits<32, DT, ND>(raw, a.flip, qd, qs);
     }
+    if (wave == 0) keep(0, bl);
+    if (count > 0) put(0);
+    if (STAGE < count) fetch(STAGE, [&](int t, int which) { return which ? lane_of(bl.v, t) : lane_of(bl.k, t); });
     __syncthreads();
-    const int D = a.c.D;
-    for (int i = threadIdx.x; i < nr * D; i += blockDim.x) {
-        const int rr = i / D, d = i - rr * D;
-        float m = -__builtin_inff();
-        for (int w = 0; w < W; ++w) m = fmaxf(m, sm[(w * a.rows_cap + rr) * 2]);
-        float o = 0.0f, l = 0.0f;
-        for (int w = 0; w < W; ++w) {
-            const float mw = sm[(w * a.rows_cap + rr) * 2];
-            const float f = mw == m ? 1.0f : __builtin_amdgcn_exp2f(mw - m);
-            l = __builtin_fmaf(f, sm[(w * a.rows_cap + rr) * 2 + 1], l);
-            o = __builtin_fmaf(f, so[((size_t)w * a.rows_cap + rr) * D + d], o);
+    for (int t = 0; t < count; t += STAGE) {
+        const int buf = (t / STAGE) & 1;
+        if (t + STAGE < count) put(buf ^ 1);
+        if (t + 2 * STAGE < count) fetch(t + 2 * STAGE, ring_block);
+        if (wave == 0) {
+            const int from = (t & ~63) + 64, at = t & 63;
+            if (from < count) {
+                if (at == 0) page = look(from);
+                if (at == STAGE) bl = find(from, page);
+                if (at == 2 * STAGE) keep(from, bl);
+            }
         }
-        const int orow = s.row0 + (r0 + rr) / a.G, ohead = kvh * a.G + (r0 + rr) % a.G;
-        if (g.n == 1) {
-            float y = l == 0.0f ? 0.0f : o / l;
-            if (failed) y = __uint_as_float(0x7FC00000u);
-            store1(a.out, a.type, (int64_t)orow * a.out_stride + (int64_t)ohead * D + d, y);
-        } else {
-            const int64_t at = (int64_t)blockIdx.x * a.rows_cap + rr;
-            a.part_o[at * D + d] = o;
-            if (d == 0) a.part_ml[at * 2] = m, a.part_ml[at * 2 + 1] = l;
+#pragma unroll
+        for (int b = 0; b < STAGE; ++b) {
+            const int t0 = (first + t + b) * KV_BLOCK;
+            if (t + b >= count || t0 >= some_hi || t0 + KV_BLOCK <= some_lo) continue;
+            const float ks = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(ring[(t + b) & 127].ks)));
+            const float vs = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(ring[(t + b) & 127].vs)));
+            const uint8_t* from = lds + buf * BUF + b * (KB + VB);
+            Keys<32, DT> k;
+#pragma unroll
+            for (int j = 0; j < DT; ++j) k[0][j] = *reinterpret_cast<const v4i*>(from + j * 1024 + lane * 16);
+            Scores<32, DT, ND> acc;
+            scores<32, DT, ND>(acc, qd, k);
+            const auto w = weights<32, DT, ND, EXT>(cy, a, acc, qs, slope, pos, ks, vs, t0, gl, lo, hi,
+                                                    t0 < whole_lo || t0 + KV_BLOCK > whole_hi);
+            const h8* v = reinterpret_cast<const h8*>(from + KB) + lane;
+#pragma unroll
+            for (int i = 0; i < DT; ++i) {
+                const h8 v0 = v[i * 128], v1 = v[i * 128 + 64];
+                cy.o[i] = value_mfma<32>(v0, w.p[0], cy.o[i]);
+                cy.o[i] = value_mfma<32>(v1, w.p[1], cy.o[i]);
+                if constexpr (ND == 3) {
+                    cy.o[i] = value_mfma<32>(v0, w.e[0], cy.o[i]);
+                    cy.o[i] = value_mfma<32>(v1, w.e[1], cy.o[i]);
+                }
+            }
         }
+        __syncthreads();
+    }
+    cy.l = row_sum<32>(cy.l);
+    if (w0 + col >= r0 + nr) return;
+    if (g.n == 1) {
+        const float f = failed ? __uint_as_float(0x7FC00000u) : cy.l == 0.0f ? 0.0f : cy.R / cy.l;
+        put_out(cy, a, (int64_t)row * a.out_stride + (int64_t)head * a.c.D, gl, f);
+    } else {
+        const int64_t p = (((int64_t)(seq * a.splits + split) * a.row_tiles + rt) * a.c.H + kvh) * a.rows_cap + 32 * wave + col;
+        put_sums(cy, a.part_o + p * a.c.D, gl, cy.R);
+        if (gl == 0) reinterpret_cast<float2*>(a.part_ml)[p] = make_float2(cy.m, cy.l);
     }
 }
 
@@ -690,7 +833,6 @@ __device__ __forceinline__ void join_row(const AttendArgs& a, int n, int rr, int
 }
 
 // Rows that k_attend divided.  blockIdx.x as there without the splits, blockIdx.y = row of the row tile.
-template <int NR>
 __global__ __launch_bounds__(256) void k_attend_join(const AttendArgs a) {
     int item = blockIdx.x;
     const int kvh = item % a.c.H;
@@ -698,9 +840,9 @@ __global__ __launch_bounds__(256) void k_attend_join(const AttendArgs a) {
     const int rt = item % a.row_tiles, seq = item / a.row_tiles;
     const int failed = *a.c.status;
     const KvSeq s = kv_seq(a.c, a.b, seq);
-    const int rows = s.n * a.G, r = rt * NR + blockIdx.y;
+    const int rows = s.n * a.G, r = rt * a.tile_rows + blockIdx.y;
     if (r >= rows) return;
-    const Range g = range_of(a, s, rt * NR, min(NR, rows - rt * NR));
+    const Range g = range_of(a, s, rt * a.tile_rows, min(a.tile_rows, rows - rt * a.tile_rows));
     if (g.n == 1) return;
     const int64_t to = (int64_t)(s.row0 + r / a.G) * a.out_stride + (int64_t)(kvh * a.G + r % a.G) * a.c.D;
     join_row<4>(a, g.n, blockIdx.y, to, failed,
@@ -897,33 +1039,34 @@ __global__ __launch_bounds__(256) void k_attend_stream_join(const AttendArgs a) 
     }
 }
 
-template <int NR, int DT>
-void launch_form(const AttendArgs& a, hipStream_t st) {
-    const bool ext = a.cap > 0.0f || a.alibi, wide = a.type == JX_TYPE_F32;
-    if (a.waves) {
-        auto k = wide ? (ext ? k_attend_stream<NR, DT, 3, true> : k_attend_stream<NR, DT, 3, false>)
-                      : (ext ? k_attend_stream<NR, DT, 2, true> : k_attend_stream<NR, DT, 2, false>);
-        const size_t lds = a.group == 1 ? 0 : stream_lds(a.rows_cap, a.c.D);
-        if (lds > 65536 - 8192)
-            (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-        hipLaunchKernelGGL(k, dim3(a.waves / 4), dim3(256), lds, st, a);
-        return;
-    }
-    const size_t lds = sizeof(float) * (size_t)waves_of(DT) * a.rows_cap * (a.c.D + 2);
-    const dim3 grid((unsigned)((int64_t)a.b.n_seqs * a.splits * a.row_tiles * a.c.H));
-    auto k = wide ? (ext ? k_attend<NR, DT, 3, true> : k_attend<NR, DT, 3, false>) : (ext ? k_attend<NR, DT, 2, true> : k_attend<NR, DT, 2, false>);
-    if (lds > 65536)
+template <typename K>
+void launch_k(K k, unsigned grid, int threads, size_t lds, const AttendArgs& a, hipStream_t st) {
+    if (lds > 48 * 1024)
         (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    hipLaunchKernelGGL(k, grid, dim3(64 * waves_of(DT)), lds, st, a);
-    if (a.splits > 1)
-        hipLaunchKernelGGL(k_attend_join<NR>, dim3((unsigned)((int64_t)a.b.n_seqs * a.row_tiles * a.c.H), a.rows_cap), dim3(256), 0, st, a);
+    hipLaunchKernelGGL(k, dim3(grid), dim3(threads), lds, st, a);
+}
+#define JX_ATTEND_FORM(kernel, ...)                                                       \
+    (wide ? (ext ? kernel<__VA_ARGS__, 3, true> : kernel<__VA_ARGS__, 3, false>)          \
+          : (ext ? kernel<__VA_ARGS__, 2, true> : kernel<__VA_ARGS__, 2, false>))
+
+template <int NR, int DT>
+void launch_form(const AttendArgs& a, bool ext, bool wide, hipStream_t st) {
+    if (a.waves)
+        launch_k(JX_ATTEND_FORM(k_attend_stream, NR, DT), a.waves / 4, 256, a.group == 1 ? 0 : stream_lds(a.rows_cap, a.c.D), a, st);
+    else
+        launch_k(JX_ATTEND_FORM(k_attend, NR, DT), (unsigned)(a.b.n_seqs * a.c.H), 64 * waves_of(DT),
+                 sizeof(float) * (size_t)waves_of(DT) * a.rows_cap * (a.c.D + 2), a, st);
 }
 template <int DT>
 void launch_dt(const AttendArgs& a, hipStream_t st) {
-    if (a.rows_cap <= 16)
-        launch_form<16, DT>(a, st);
+    const bool ext = a.cap > 0.0f || a.alibi, wide = a.type == JX_TYPE_F32;
+    if (a.tile_rows > 32)
+        launch_k(JX_ATTEND_FORM(k_attend_rows, DT), (unsigned)((int64_t)a.b.n_seqs * a.splits * a.row_tiles * a.c.H), 64 * rows_waves(DT),
+                 (size_t)2 * STAGE * 3072 * DT, a, st);
+    else if (a.rows_cap <= 16)
+        launch_form<16, DT>(a, ext, wide, st);
     else
-        launch_form<32, DT>(a, st);
+        launch_form<32, DT>(a, ext, wide, st);
 }
 
 }  // namespace
@@ -931,32 +1074,39 @@ void launch_dt(const AttendArgs& a, hipStream_t st) {
 AttendPlan attend_plan(const jx_kv_cache& c, const jx_kv_batch& b, const jx_attention& t) {
     AttendPlan p;
     const int64_t most = (int64_t)c.max_pages * c.page_tokens;
-    const int G = t.n_heads / c.n_kv_heads, W = waves_of(c.head_dim / 32);
-    p.row_tiles = (int)(((int64_t)b.max_rows * G + 31) / 32);
-    p.rows_cap = (int)std::min<int64_t>(32, (int64_t)b.max_rows * G);
+    const int G = t.n_heads / c.n_kv_heads, DT = c.head_dim / 32, W = waves_of(DT);
+    const int64_t rows = (int64_t)b.max_rows * G;
     int64_t len = b.max_len > 0 ? std::min<int64_t>(b.max_len, most) : most;
     if (t.window > 0 && t.causal) len = std::min<int64_t>(len, (int64_t)t.window + b.max_rows + KV_BLOCK);
     const int64_t tiles = std::max<int64_t>(1, (len + KV_BLOCK - 1) / KV_BLOCK);
-    const int64_t items = (int64_t)b.n_seqs * p.row_tiles * c.n_kv_heads;
+    // a line of the batch's tiles has its places in 32 bits
+    const bool line = (int64_t)b.n_seqs * c.n_kv_heads * ((most + KV_BLOCK - 1) / KV_BLOCK + START) < INT32_MAX;
     p.splits = 1;
     p.chunk = (int)tiles;
     p.waves = 0;
     p.group = 1;
     p.partials = 0;
-    if (p.row_tiles == 1 && !(items <= 256 && tiles <= 4 * W) &&
-        (int64_t)b.n_seqs * c.n_kv_heads * ((most + KV_BLOCK - 1) / KV_BLOCK) < INT32_MAX) {
-        // as many waves as are resident at once: registers, and 160 KB of LDS less the workgroup's fixed 7
-        const size_t lds = stream_lds(p.rows_cap, c.head_dim);
+    if (rows <= 32 && line) {
+        const int64_t items = (int64_t)b.n_seqs * c.n_kv_heads;
+        p.tile_rows = 32;
+        p.row_tiles = 1;
+        p.rows_cap = (int)rows;
+        if (items <= 256 && tiles <= 4 * W) return p;  // a workgroup for each sequence and kv head, four tiles per wave at most
         // few sequences and heads have many parts each: 8 of them 57 us with a group's parts joined and 58 without, 64 (draft
         // tokens, 10 rows of 256 dimensions) 32 and 33; 272 and 512 of them 22 and 21, 60 and 58
+        const size_t lds = stream_lds(p.rows_cap, c.head_dim);
         p.group = items <= 128 && lds <= 150 * 1024 ? 4 : 1;
-        const int by_registers = stream_occupancy(p.rows_cap <= 16 ? 16 : 32, c.head_dim / 32);
-        p.waves = 256 * 4 * (p.group == 4 && lds > 72 * 1024 ? 1 : by_registers);
+        // as many waves as are resident at once: registers, and 160 KB of LDS less the workgroup's fixed 7
+        p.waves = 256 * 4 * (p.group == 4 && lds > 72 * 1024 ? 1 : stream_occupancy(rows <= 16 ? 16 : 32, DT));
         p.partials = 2 * (int64_t)p.waves;
         return p;
     }
-    // about two workgroups for each of the 256 CUs, of at least two tiles per wave
-    const int64_t splits = std::max<int64_t>(1, std::min<int64_t>(512 / std::max<int64_t>(1, items), tiles / (2 * W)));
+    p.tile_rows = 32 * rows_waves(DT);
+    p.row_tiles = (int)((rows + p.tile_rows - 1) / p.tile_rows);
+    p.rows_cap = (int)std::min<int64_t>(p.tile_rows, rows);
+    const int64_t items = (int64_t)b.n_seqs * p.row_tiles * c.n_kv_heads;
+    // a workgroup for each of the 256 CUs, of at least 16 tiles
+    const int64_t splits = std::max<int64_t>(1, std::min<int64_t>(256 / std::max<int64_t>(1, items), tiles / 16));
     p.chunk = (int)((tiles + splits - 1) / splits);
     p.splits = (int)((tiles + p.chunk - 1) / p.chunk);
     if (p.splits > 1) p.partials = items * p.splits;
@@ -974,10 +1124,11 @@ void launch_attend(const AttendArgs& a, hipStream_t st) {
         case 7: launch_dt<7>(a, st); break;
         default: launch_dt<8>(a, st); break;
     }
-    if (a.waves)
-        // few sequences and heads: a workgroup per row (many partials each); many: one for all rows
-        hipLaunchKernelGGL(k_attend_stream_join, dim3((unsigned)((int64_t)a.b.n_seqs * a.c.H), (int64_t)a.b.n_seqs * a.c.H <= 128 ? a.rows_cap : 1),
-                           dim3(256), 0, st, a);
+    const unsigned pairs = (unsigned)(a.b.n_seqs * a.c.H);
+    if (a.waves)  // few sequences and heads: a workgroup per row (many partials each); many: one for all rows
+        hipLaunchKernelGGL(k_attend_stream_join, dim3(pairs, pairs <= 128 ? a.rows_cap : 1), dim3(256), 0, st, a);
+    else if (a.splits > 1)
+        hipLaunchKernelGGL(k_attend_join, dim3(pairs * a.row_tiles, a.rows_cap), dim3(256), 0, st, a);
 }
 
 }  // namespace jx

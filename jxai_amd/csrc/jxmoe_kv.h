@@ -65,22 +65,24 @@ struct AttendArgs {
     float* part_o;   // [partials][rows_cap][D] sums of weights times values
     float* part_ml;  // [partials][rows_cap][2] the running maximum and the sum of weights
     int type, heads, G;
-    float scale2;    // scale * log2(e)
+    float scale;     // |softmax scale|
+    float scale2;    // |softmax scale| * log2(e)
+    bool flip;       // it is negative
     float cap;       // 0: none (natural units)
-    float scale;
     int window, causal;
     int chunk;       // tiles of 32 tokens that a workgroup takes at most, unless that makes more than `splits` of a sequence
     int splits;
     int waves;       // k_attend_stream: waves of the launch
     int group;       //   waves whose parts become one partial
+    int tile_rows;   // rows of a row tile; more than 32: k_attend_rows
     int row_tiles;   // of the sequence with the most rows
-    int rows_cap;    // rows of a row tile at most: min(tile, max_rows * G)
+    int rows_cap;    // rows of a row tile at most: min(tile_rows, max_rows * G)
     bool q_vec, out_vec;  // 16-byte aligned rows
 };
 
 // How many splits the launch for this batch takes, and its chunk; the workspace is sized by it.
 struct AttendPlan {
-    int splits, chunk, row_tiles, rows_cap;
+    int splits, chunk, tile_rows, row_tiles, rows_cap;
     int waves, group;  // waves not 0: k_attend_stream
     int64_t partials;  // of the workspace, each rows_cap rows of D + 2 floats
 };

@@ -1,6 +1,7 @@
 // The paged 8-bit key/value cache: new tokens into it, its pages (reserve, trim, fork, compact), and the C entry points of the
 // cache and its attention.
 #include <algorithm>
+#include <cmath>
 
 #include "jxmoe_device.h"
 #include "jxmoe_kv.h"
@@ -796,8 +797,9 @@ int jx_kv_attention(const jx_kv_cache* c, const jx_kv_batch* b, const jx_attenti
     a.type = t->type;
     a.heads = t->n_heads;
     a.G = t->n_heads / c->n_kv_heads;
-    a.scale = t->scale;
-    a.scale2 = t->scale * 1.44269504088896340736f;
+    a.scale = std::fabs(t->scale);
+    a.scale2 = a.scale * 1.44269504088896340736f;
+    a.flip = std::signbit(t->scale);
     a.cap = t->softcap;
     a.window = std::min(t->window, KV_MAX_TOKENS);
     a.causal = t->causal;
@@ -805,6 +807,7 @@ int jx_kv_attention(const jx_kv_cache* c, const jx_kv_batch* b, const jx_attenti
     a.splits = p.splits;
     a.waves = p.waves;
     a.group = p.group;
+    a.tile_rows = p.tile_rows;
     a.row_tiles = p.row_tiles;
     a.rows_cap = p.rows_cap;
     a.q_vec = aligned(q, 16) && a.q_stride * size % 16 == 0;
