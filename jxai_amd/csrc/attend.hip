@@ -20,6 +20,7 @@ namespace {
 
 constexpr float LOG2E = 1.44269504088896340736f;
 constexpr int OFF = 9;        // weights are held times 2^OFF: fp16's full precision down to 2^-23 of the reference
+constexpr float LOWEST = -3e38f;  // the reference of a row that has seen nothing: finite, so that differences are numbers
 constexpr float LAG = 6.0f;   // the reference maximum follows when it is 2^LAG behind: 2^(OFF + LAG) < 65504
 
 __device__ __forceinline__ float load1(const void* p, int type, int64_t i) {
@@ -237,6 +238,30 @@ __device__ __forceinline__ void digits(const Raw<NR, DT>& v, bool flip, Digits<N
         }
 }
 
+// The same as one (fp32: two) fp16 values each, with the row's largest between 2^4 and 2^5: the form for K in fp16 (k_attend_rows).
+// F16 and BF16 are held whole, except below 2^-18 of the row's largest; fp32 in 22 bits.  piece u of step j: dimensions 8 u .. + 7
+template <int DT, int ND>
+__device__ __forceinline__ void halves(const Raw<32, DT>& v, bool flip, h8 (&qh)[ND - 1][DT][2], float& qs) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < DT; ++j)
+#pragma unroll
+        for (int k = 0; k < 16; ++k) top = max(top, __float_as_uint(v[j][k]) & 0x7FFFFFFFu);
+    top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
+    const bool finite = top < 0x7F800000u, zero = top < 0x0D800000u;
+    const int e = (int)(top >> 23) - 127 - 4;  // the row in units of 2^e
+    const float inv = finite && !zero ? __uint_as_float((uint32_t)(127 - e) << 23) : 0.0f;
+    qs = !finite ? __uint_as_float(0x7FC00000u) : zero ? 0.0f : __uint_as_float((uint32_t)(127 + e) << 23);
+#pragma unroll
+    for (int j = 0; j < DT; ++j)
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+            const float u = v[j][k] * (flip ? -inv : inv);
+            qh[0][j][k >> 3][k & 7] = (_Float16)u;
+            if constexpr (ND == 3) qh[1][j][k >> 3][k & 7] = (_Float16)(u - (float)(_Float16)u);
+        }
+}
+
 // What a wave carries for its rows.
 template <int NR, int DT>
 struct Carry {
@@ -249,7 +274,7 @@ template <int NR, int DT>
 __device__ __forceinline__ void carry_init(Carry<NR, DT>& s) {
 #pragma unroll
     for (auto& o : s.o) o = typename Form<NR, DT>::Out{};
-    s.m = -__builtin_inff();
+    s.m = LOWEST;
     s.l = 0.0f;
     s.R = 0.0f;
 }
@@ -291,13 +316,11 @@ struct Weights {
     h8 p[NR / 16], e[ND == 3 ? NR / 16 : 1];
 };
 
-// From S^T of a block whose tokens begin at t0.  lo / hi: the lane's row sees tokens lo .. hi - 1 (masked: whether to look).
-template <int NR, int DT, int ND, bool EXT>
-__device__ __forceinline__ Weights<NR, ND> weights(Carry<NR, DT>& s, const AttendArgs& a, const Scores<NR, DT, ND>& acc, float qs, float slope,
-                                                   int pos, float ks, float vs, int t0, int g, int lo, int hi, bool masked) {
+// S^T as floats in units of the last digit
+template <int NR, int DT, int ND>
+__device__ __forceinline__ void score_values(const Scores<NR, DT, ND>& acc, float (&x)[Form<NR, DT>::X]) {
     typedef Form<NR, DT> F;
     constexpr int X = F::X, PER = X / F::ACCS;
-    float x[X];
 #pragma unroll
     for (int i = 0; i < X; ++i) {
         const int t = i / PER, k = i % PER;
@@ -307,6 +330,15 @@ __device__ __forceinline__ Weights<NR, ND> weights(Carry<NR, DT>& s, const Atten
         else
             x[i] = __builtin_fmaf((float)acc[0][t][k], 16384.0f, (float)(int)(((uint32_t)acc[1][t][k] << 7) + (uint32_t)acc[2][t][k]));
     }
+}
+
+// From the scores x (in units of qs * ks) of a block whose tokens begin at t0.  lo / hi: the lane's row sees tokens lo .. hi - 1
+// (masked: whether to look).  before(): runs ahead of the exponentials.
+template <int NR, int DT, int ND, bool EXT, typename B>
+__device__ __forceinline__ Weights<NR, ND> weights(Carry<NR, DT>& s, const AttendArgs& a, float (&x)[Form<NR, DT>::X], float qs, float slope,
+                                                   int pos, float ks, float vs, int t0, int g, int lo, int hi, bool masked, B before) {
+    typedef Form<NR, DT> F;
+    constexpr int X = F::X;
     // x * c is the exponent of 2.  (c is kept above 0, so that a masked -inf stays what it is; the sign of the softmax scale is in q.)
     float c = qs * ks * (EXT ? a.scale : a.scale2);
     c = c < 1e-30f ? 1e-30f : c;
@@ -320,8 +352,8 @@ __device__ __forceinline__ Weights<NR, ND> weights(Carry<NR, DT>& s, const Atten
         }
         c = LOG2E;
     }
-    const int l0 = lo - t0 - 4 * g, h0 = hi - t0 - 4 * g;
     if (masked) {
+        const int l0 = lo - t0 - 4 * g, h0 = hi - t0 - 4 * g;
 #pragma unroll
         for (int i = 0; i < X; ++i) x[i] = F::token(i) >= l0 && F::token(i) < h0 ? x[i] : -__builtin_inff();
     }
@@ -330,38 +362,35 @@ __device__ __forceinline__ Weights<NR, ND> weights(Carry<NR, DT>& s, const Atten
     for (int i = 1; i < X; ++i) top = fmaxf(top, x[i]);
     top = row_max<NR>(top) * c;
     if (__any(top > s.m + LAG)) {
-        const float m = fmaxf(s.m, top);
-        const float f = m == s.m ? 1.0f : __builtin_amdgcn_exp2f(s.m - m);
+        const float m = fmaxf(s.m, top), f = __builtin_amdgcn_exp2f(s.m - m);
         s.m = m;
         s.l *= f;
         carry_scale(s, f);
     }
-    if (vs > s.R) {
-        carry_scale(s, s.R / vs);
-        s.R = vs;
+    // V's scale relative to R goes into the exponent and out of the sum again.  (A block of zeros, whose scale is 0, may weigh
+    // anything; 2^-100 of R is far below what the weights' fp16 holds.)
+    if (!(vs <= s.R)) {
+        if (vs > s.R) {
+            carry_scale(s, s.R * __builtin_amdgcn_rcpf(vs));
+            s.R = vs;
+        } else {  // NaN: so is every row that sees a token of the block
+            bool sees = !masked;
+#pragma unroll
+            for (int i = 0; i < X; ++i) sees |= x[i] != -__builtin_inff();
+            s.l += sees ? vs : 0.0f;
+            vs = 0.0f;
+        }
     }
-    // V's scale goes into the exponent and out of the sum again where it is not too small beside R; otherwise (a block of
-    // zeros has scale 0, and NaN marks one that reads as NaN) into the weights behind the sum.
-    const float vr = vs == s.R && vs > 0.0f ? 1.0f : vs == 0.0f ? 0.0f : vs / s.R;
-    const bool near = vr >= 0x1p-20f;
-    const float ref = (s.m == -__builtin_inff() ? 0.0f : s.m) - (float)OFF - (near ? __builtin_amdgcn_logf(vr) : 0.0f);
+    const float vr = vs == 0.0f ? 1.0f : fmaxf(vs * __builtin_amdgcn_rcpf(s.R), 0x1p-100f);
+    const float ref = s.m - ((float)OFF + __builtin_amdgcn_logf(vr));
+    before();
     float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < X; ++i) {
         x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], c, -ref));
         sum += x[i];
     }
-    if (near) {
-        s.l = __builtin_fmaf(sum, __builtin_amdgcn_rcpf(vr), s.l);
-    } else {
-        s.l += sum;
-#pragma unroll
-        for (int i = 0; i < X; ++i) x[i] *= vr;
-        if (masked) {  // nothing of a NaN scale reaches a row that does not see the block
-#pragma unroll
-            for (int i = 0; i < X; ++i) x[i] = F::token(i) >= l0 && F::token(i) < h0 ? x[i] : 0.0f;
-        }
-    }
+    s.l = __builtin_fmaf(sum, __builtin_amdgcn_rcpf(vr), s.l);
     // 32 rows: token 8 a + 4 g + b is register 4 a + b here and byte 8 (a & 1) + 4 (a >> 1) + b of V.  16 rows: in order
     Weights<NR, ND> w;
 #pragma unroll
@@ -503,8 +532,10 @@ __device__ __forceinline__ void attend_tiles(Carry<NR, DT>& cy, const AttendArgs
             scores<NR, DT, ND>(acc, qd, k);
             if (i + 1 < n) fetch_k(i + 1);
             const int t0 = (first + (b0 + i) * step) * KV_BLOCK;
-            const auto w = weights<NR, DT, ND, EXT>(cy, a, acc, qs, slope, pos, lane_of(bl.ks, i), lane_of(bl.vs, i), t0, g, lo, hi,
-                                                    t0 < whole_lo || t0 + KV_BLOCK > whole_hi);
+            float x[F::X];
+            score_values<NR, DT, ND>(acc, x);
+            const auto w = weights<NR, DT, ND, EXT>(cy, a, x, qs, slope, pos, lane_of(bl.ks, i), lane_of(bl.vs, i), t0, g, lo, hi,
+                                                    t0 < whole_lo || t0 + KV_BLOCK > whole_hi, [] {});
             add_values<NR, DT, ND>(cy, w, v);
             if (i + 1 < n) fetch_v(i + 1);
         }
@@ -609,17 +640,21 @@ __global__ __launch_bounds__(64 * waves_of(DT)) void k_attend(const AttendArgs a
 // ---------------------------------------------------------------- many rows: K and V through LDS
 
 constexpr int rows_waves(int dt) { return dt <= 4 ? 8 : 4; }  // (more than 128 dimensions: one wave per SIMD)
-constexpr int STAGE = 2;                                      // blocks of 32 tokens in LDS at a time
+constexpr int rows_stage(int dt) { return dt <= 4 ? 2 : 1; }  // blocks of 32 tokens that are staged at a time
+constexpr int BUFS = 3;
 
-// 32 rows per wave, 8 (4) waves against the same blocks.  A stage of two blocks goes through registers into one of two LDS
-// buffers: K's codes as they are, V's as fp16 in the order that the products read (converted once for all waves).  Both are
-// read and written 16 bytes per lane in a row.  While a stage is worked on, the next one is written and the one behind
-// it loaded; one barrier per stage.
+// 32 rows per wave, 8 (4) waves against the same blocks.  A stage of two blocks (one) goes through registers into one of three
+// LDS buffers as fp16, K and V in the order that the products read (16 bytes per lane in a row), converted once for all waves.
+// While a stage is worked on, the one behind the next is written and the one behind that loaded; one barrier per stage.  A
+// block's K is read from LDS during the block before (all waves ask for K behind a barrier at once otherwise), its V
+// while its weights are formed.
+// K Q^T is fp16 here, not digits: the vector unit is what bounds the loop, and joining and converting two digits' sums costs
+// it 32 of about 150 instructions per block.
 // blockIdx.x = ((sequence * splits + split) * row_tiles + row tile from the last) * H + kv head: the longest rows of a
 // causal prompt first, and the row tiles of 8 kv heads each on an XCD of their own, whose L2 keeps the head's K and V.
 template <int DT, int ND, bool EXT>
 __global__ __launch_bounds__(64 * rows_waves(DT), DT <= 4 ? 2 : 1) void k_attend_rows(const AttendArgs a) {
-    constexpr int W = rows_waves(DT), KB = 1024 * DT, VB = 2048 * DT, BUF = STAGE * (KB + VB);
+    constexpr int W = rows_waves(DT), STAGE = rows_stage(DT), KB = 1024 * DT, HB = 2 * KB, BUF = STAGE * 2 * HB;  // bytes of a block, in fp16, of a buffer
     constexpr int LOADS = (2 * STAGE * DT + W - 1) / W;  // of 1 KB per wave and stage
     extern __shared__ uint4 lds4[];
     __shared__ Blocks ring[128];
@@ -669,14 +704,11 @@ __global__ __launch_bounds__(64 * rows_waves(DT), DT <= 4 ? 2 : 1) void k_attend
             const int u = wave + i * W;
             if (u >= 2 * STAGE * DT) break;
             const int which = u >= STAGE * DT, v = u - which * STAGE * DT, b = v / DT, kb = v % DT;
-            if (!which) {
-                *reinterpret_cast<uint4*>(to + b * (KB + VB) + kb * 1024 + lane * 16) = in[i];
-            } else {  // the lane's 16 bytes are piece (h, d): tokens of the first and of the second product
-                const int piece = kb * 64 + lane, h = piece / (32 * DT), d = piece % (32 * DT);
-                h8* o = reinterpret_cast<h8*>(to + b * (KB + VB) + KB) + (d >> 5) * 128 + h * 32 + (d & 31);
-                o[0] = codes_to_half(in[i].x, in[i].y);
-                o[64] = codes_to_half(in[i].z, in[i].w);
-            }
+            // K: the lane's 16 bytes are dimensions 16 h .. of step kb; V: piece (h, d).  Eight for each of two products
+            const int piece = kb * 64 + lane, h = piece / (32 * DT), d = piece % (32 * DT);
+            h8* o = reinterpret_cast<h8*>(to + (2 * b + which) * HB) + (which ? (d >> 5) * 128 + h * 32 + (d & 31) : kb * 128 + lane);
+            o[0] = codes_to_half(in[i].x, in[i].y);
+            o[64] = codes_to_half(in[i].z, in[i].w);
         }
     };
     // blocks and scales of 128 tiles around the current one: wave 0 looks the next 64 up, a step per stage
@@ -685,7 +717,7 @@ __global__ __launch_bounds__(64 * rows_waves(DT), DT <= 4 ? 2 : 1) void k_attend
     auto look = [&](int t) { return page_of(a, s.slot, first + t + lane, t + lane < count); };
     auto find = [&](int t, int page) { return blocks_of(a, kvh, page, first + t + lane, t + lane < count); };
 
-    Digits<32, DT, ND> qd;
+    h8 qh[ND - 1][DT][2];
     float qs, slope = 0.0f;
     int page = look(0);
     Blocks bl;
@@ -695,16 +727,30 @@ __global__ __launch_bounds__(64 * rows_waves(DT), DT <= 4 ? 2 : 1) void k_attend
         if (EXT && a.alibi) slope = a.alibi[head];
         bl = find(0, page);
         if (count > 0) fetch(0, [&](int t, int which) { return which ? lane_of(bl.v, t) : lane_of(bl.k, t); });
-        digits<32, DT, ND>(raw, a.flip, qd, qs);
+        halves<DT, ND>(raw, a.flip, qh, qs);
     }
+    auto first_block = [&](int t, int which) { return which ? lane_of(bl.v, t) : lane_of(bl.k, t); };
     if (wave == 0) keep(0, bl);
     if (count > 0) put(0);
-    if (STAGE < count) fetch(STAGE, [&](int t, int which) { return which ? lane_of(bl.v, t) : lane_of(bl.k, t); });
+    if (STAGE < count) {
+        fetch(STAGE, first_block);
+        put(1);
+    }
+    if (2 * STAGE < count) fetch(2 * STAGE, first_block);
     __syncthreads();
+    h8 k[2 * DT];
+    auto key = [&](const uint8_t* block) {
+#pragma unroll
+        for (int j = 0; j < 2 * DT; ++j) k[j] = reinterpret_cast<const h8*>(block)[j * 64 + lane];
+    };
+    constexpr bool EARLY = DT <= 6;      // (more dimensions: K at its block's beginning, the registers are needed)
+    constexpr int VH = EARLY ? 2 * DT : 6;  // pieces of V ahead of the exponentials
+    if (EARLY) key(lds);
+    int buf = 0;  // of the stage, and of the two behind it
     for (int t = 0; t < count; t += STAGE) {
-        const int buf = (t / STAGE) & 1;
-        if (t + STAGE < count) put(buf ^ 1);
-        if (t + 2 * STAGE < count) fetch(t + 2 * STAGE, ring_block);
+        const int buf1 = buf == BUFS - 1 ? 0 : buf + 1, buf2 = buf1 == BUFS - 1 ? 0 : buf1 + 1;
+        if (t + 2 * STAGE < count) put(buf2);
+        if (t + 3 * STAGE < count) fetch(t + 3 * STAGE, ring_block);
         if (wave == 0) {
             const int from = (t & ~63) + 64, at = t & 63;
             if (from < count) {
@@ -715,30 +761,47 @@ __global__ __launch_bounds__(64 * rows_waves(DT), DT <= 4 ? 2 : 1) void k_attend
         }
 #pragma unroll
         for (int b = 0; b < STAGE; ++b) {
+            if (t + b >= count) break;
             const int t0 = (first + t + b) * KV_BLOCK;
-            if (t + b >= count || t0 >= some_hi || t0 + KV_BLOCK <= some_lo) continue;
+            const uint8_t* block = lds + buf * BUF + 2 * b * HB;
+            const uint8_t* next = b + 1 < STAGE ? block + 2 * HB : lds + buf1 * BUF;  // (behind the last block: what is there)
+            if (t0 >= some_hi || t0 + KV_BLOCK <= some_lo) {
+                if (EARLY) key(next);
+                continue;
+            }
+            if (!EARLY) key(block);
             const float ks = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(ring[(t + b) & 127].ks)));
             const float vs = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(ring[(t + b) & 127].vs)));
-            const uint8_t* from = lds + buf * BUF + b * (KB + VB);
-            Keys<32, DT> k;
+            v16f acc = {};
 #pragma unroll
-            for (int j = 0; j < DT; ++j) k[0][j] = *reinterpret_cast<const v4i*>(from + j * 1024 + lane * 16);
-            Scores<32, DT, ND> acc;
-            scores<32, DT, ND>(acc, qd, k);
-            const auto w = weights<32, DT, ND, EXT>(cy, a, acc, qs, slope, pos, ks, vs, t0, gl, lo, hi,
-                                                    t0 < whole_lo || t0 + KV_BLOCK > whole_hi);
-            const h8* v = reinterpret_cast<const h8*>(from + KB) + lane;
+            for (int j = 0; j < 2 * DT; ++j) {
+                acc = value_mfma<32>(k[j], qh[0][j >> 1][j & 1], acc);
+                if constexpr (ND == 3) acc = value_mfma<32>(k[j], qh[1][j >> 1][j & 1], acc);
+            }
+            float x[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = acc[i];
+            h8 v[2 * DT];
+            const h8* value = reinterpret_cast<const h8*>(block + HB) + lane;
+            const auto w = weights<32, DT, ND, EXT>(cy, a, x, qs, slope, pos, ks, vs, t0, gl, lo, hi,
+                                                    t0 < whole_lo || t0 + KV_BLOCK > whole_hi, [&] {
+#pragma unroll
+                                                        for (int i = 0; i < VH; ++i) v[i] = value[i * 64];
+                                                        if (EARLY) key(next);
+                                                        __builtin_amdgcn_sched_barrier(0);
+                                                    });
 #pragma unroll
             for (int i = 0; i < DT; ++i) {
-                const h8 v0 = v[i * 128], v1 = v[i * 128 + 64];
-                cy.o[i] = value_mfma<32>(v0, w.p[0], cy.o[i]);
-                cy.o[i] = value_mfma<32>(v1, w.p[1], cy.o[i]);
+                if (2 * i + VH < 2 * DT) v[2 * i + VH] = value[(2 * i + VH) * 64], v[2 * i + VH + 1] = value[(2 * i + VH + 1) * 64];
+                cy.o[i] = value_mfma<32>(v[2 * i], w.p[0], cy.o[i]);
+                cy.o[i] = value_mfma<32>(v[2 * i + 1], w.p[1], cy.o[i]);
                 if constexpr (ND == 3) {
-                    cy.o[i] = value_mfma<32>(v0, w.e[0], cy.o[i]);
-                    cy.o[i] = value_mfma<32>(v1, w.e[1], cy.o[i]);
+                    cy.o[i] = value_mfma<32>(v[2 * i], w.e[0], cy.o[i]);
+                    cy.o[i] = value_mfma<32>(v[2 * i + 1], w.e[1], cy.o[i]);
                 }
             }
         }
+        buf = buf1;
         __syncthreads();
     }
     cy.l = row_sum<32>(cy.l);
@@ -1062,7 +1125,7 @@ void launch_dt(const AttendArgs& a, hipStream_t st) {
     const bool ext = a.cap > 0.0f || a.alibi, wide = a.type == JX_TYPE_F32;
     if (a.tile_rows > 32)
         launch_k(JX_ATTEND_FORM(k_attend_rows, DT), (unsigned)((int64_t)a.b.n_seqs * a.splits * a.row_tiles * a.c.H), 64 * rows_waves(DT),
-                 (size_t)2 * STAGE * 3072 * DT, a, st);
+                 (size_t)BUFS * rows_stage(DT) * 4096 * DT, a, st);
     else if (a.rows_cap <= 16)
         launch_form<16, DT>(a, ext, wide, st);
     else
