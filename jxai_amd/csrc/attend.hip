@@ -332,15 +332,15 @@ __device__ __forceinline__ void score_values(const Scores<NR, DT, ND>& acc, floa
     }
 }
 
-// From the scores x (in units of qs * ks) of a block whose tokens begin at t0.  lo / hi: the lane's row sees tokens lo .. hi - 1
-// (masked: whether to look).  before(): runs ahead of the exponentials.
-template <int NR, int DT, int ND, bool EXT, typename B>
-__device__ __forceinline__ Weights<NR, ND> weights(Carry<NR, DT>& s, const AttendArgs& a, float (&x)[Form<NR, DT>::X], float qs, float slope,
-                                                   int pos, float ks, float vs, int t0, int g, int lo, int hi, bool masked, B before) {
+// The scores x (in units of qs * ks) of a block whose tokens begin at t0, capped, biased and masked: x * c is the exponent of 2
+// afterwards.  Returns the row's largest.  lo / hi: the lane's row sees tokens lo .. hi - 1 (masked: whether to look).
+template <int NR, int DT, bool EXT>
+__device__ __forceinline__ float see_scores(const AttendArgs& a, float (&x)[Form<NR, DT>::X], float& c, float qs, float slope, int pos, float ks,
+                                            int t0, int g, int lo, int hi, bool masked) {
     typedef Form<NR, DT> F;
     constexpr int X = F::X;
-    // x * c is the exponent of 2.  (c is kept above 0, so that a masked -inf stays what it is; the sign of the softmax scale is in q.)
-    float c = qs * ks * (EXT ? a.scale : a.scale2);
+    // (c is kept above 0, so that a masked -inf stays what it is; the sign of the softmax scale is in q)
+    c = qs * ks * (EXT ? a.scale : a.scale2);
     c = c < 1e-30f ? 1e-30f : c;
     if constexpr (EXT) {
         const float inv = a.cap > 0.0f ? 1.0f / a.cap : 0.0f, d0 = (float)(t0 + 4 * g - pos);
@@ -360,30 +360,44 @@ __device__ __forceinline__ Weights<NR, ND> weights(Carry<NR, DT>& s, const Atten
     float top = x[0];
 #pragma unroll
     for (int i = 1; i < X; ++i) top = fmaxf(top, x[i]);
-    top = row_max<NR>(top) * c;
+    return top * c;
+}
+
+// The reference maximum after scores up to `top` (of the lane's tokens)
+template <int NR, int DT>
+__device__ __forceinline__ void follow(Carry<NR, DT>& s, float top) {
+    top = row_max<NR>(top);
     if (__any(top > s.m + LAG)) {
         const float m = fmaxf(s.m, top), f = __builtin_amdgcn_exp2f(s.m - m);
         s.m = m;
         s.l *= f;
         carry_scale(s, f);
     }
-    // V's scale relative to R goes into the exponent and out of the sum again.  (A block of zeros, whose scale is 0, may weigh
-    // anything; 2^-100 of R is far below what the weights' fp16 holds.)
+}
+// R after a block of scale vs.  One of NaN makes every row NaN that sees a token of the block (x: its scores).
+template <int NR, int DT>
+__device__ __forceinline__ void follow_value(Carry<NR, DT>& s, const float (&x)[Form<NR, DT>::X], float& vs) {
     if (!(vs <= s.R)) {
         if (vs > s.R) {
             carry_scale(s, s.R * __builtin_amdgcn_rcpf(vs));
             s.R = vs;
-        } else {  // NaN: so is every row that sees a token of the block
-            bool sees = !masked;
+        } else {
+            bool sees = false;
 #pragma unroll
-            for (int i = 0; i < X; ++i) sees |= x[i] != -__builtin_inff();
+            for (float v : x) sees |= v != -__builtin_inff();
             s.l += sees ? vs : 0.0f;
             vs = 0.0f;
         }
     }
+}
+
+// The weights of a block.  V's scale relative to R goes into the exponent and out of the sum again.  (A block of zeros, whose
+// scale is 0, may weigh anything; 2^-100 of R is far below what the weights' fp16 holds.)
+template <int NR, int DT, int ND>
+__device__ __forceinline__ Weights<NR, ND> weights(Carry<NR, DT>& s, float (&x)[Form<NR, DT>::X], float c, float vs) {
+    constexpr int X = Form<NR, DT>::X;
     const float vr = vs == 0.0f ? 1.0f : fmaxf(vs * __builtin_amdgcn_rcpf(s.R), 0x1p-100f);
     const float ref = s.m - ((float)OFF + __builtin_amdgcn_logf(vr));
-    before();
     float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < X; ++i) {
@@ -534,8 +548,11 @@ __device__ __forceinline__ void attend_tiles(Carry<NR, DT>& cy, const AttendArgs
             const int t0 = (first + (b0 + i) * step) * KV_BLOCK;
             float x[F::X];
             score_values<NR, DT, ND>(acc, x);
-            const auto w = weights<NR, DT, ND, EXT>(cy, a, x, qs, slope, pos, lane_of(bl.ks, i), lane_of(bl.vs, i), t0, g, lo, hi,
-                                                    t0 < whole_lo || t0 + KV_BLOCK > whole_hi, [] {});
+            float c, vs = lane_of(bl.vs, i);
+            follow(cy, see_scores<NR, DT, EXT>(a, x, c, qs, slope, pos, lane_of(bl.ks, i), t0, g, lo, hi,
+                                               t0 < whole_lo || t0 + KV_BLOCK > whole_hi));
+            follow_value(cy, x, vs);
+            const auto w = weights<NR, DT, ND>(cy, x, c, vs);
             add_values<NR, DT, ND>(cy, w, v);
             if (i + 1 < n) fetch_v(i + 1);
         }
@@ -639,22 +656,19 @@ __global__ __launch_bounds__(64 * waves_of(DT)) void k_attend(const AttendArgs a
 
 // ---------------------------------------------------------------- many rows: K and V through LDS
 
-constexpr int rows_waves(int dt) { return dt <= 4 ? 8 : 4; }  // (more than 128 dimensions: one wave per SIMD)
-constexpr int rows_stage(int dt) { return dt <= 4 ? 2 : 1; }  // blocks of 32 tokens that are staged at a time
-constexpr int BUFS = 3;
+constexpr int ROWS_W = 4;  // waves; two workgroups share a CU (up to 128 dimensions)
+constexpr int STAGE = 2;   // blocks of 32 tokens in LDS at a time
 
-// 32 rows per wave, 8 (4) waves against the same blocks.  A stage of two blocks (one) goes through registers into one of three
-// LDS buffers as fp16, K and V in the order that the products read (16 bytes per lane in a row), converted once for all waves.
-// While a stage is worked on, the one behind the next is written and the one behind that loaded; one barrier per stage.  A
-// block's K is read from LDS during the block before (all waves ask for K behind a barrier at once otherwise), its V
-// while its weights are formed.
+// 32 rows per wave, four waves against the same blocks.  A stage of two blocks goes through registers into one of two LDS buffers
+// as fp16, K and V in the order that the products read (16 bytes per lane in a row), converted once for all waves.  While a
+// stage is worked on, the next one is written to LDS and the two behind that are on their way; one barrier per stage.
 // K Q^T is fp16 here, not digits: the vector unit is what bounds the loop, and joining and converting two digits' sums costs
 // it 32 of about 150 instructions per block.
 // blockIdx.x = ((sequence * splits + split) * row_tiles + row tile from the last) * H + kv head: the longest rows of a
 // causal prompt first, and the row tiles of 8 kv heads each on an XCD of their own, whose L2 keeps the head's K and V.
 template <int DT, int ND, bool EXT>
-__global__ __launch_bounds__(64 * rows_waves(DT), DT <= 4 ? 2 : 1) void k_attend_rows(const AttendArgs a) {
-    constexpr int W = rows_waves(DT), STAGE = rows_stage(DT), KB = 1024 * DT, HB = 2 * KB, BUF = STAGE * 2 * HB;  // bytes of a block, in fp16, of a buffer
+__global__ __launch_bounds__(64 * ROWS_W, DT <= 4 ? 2 : 1) void k_attend_rows(const AttendArgs a) {
+    constexpr int W = ROWS_W, KB = 1024 * DT, HB = 2 * KB, BUF = STAGE * 2 * HB;  // bytes of a block, in fp16, of a buffer
     constexpr int LOADS = (2 * STAGE * DT + W - 1) / W;  // of 1 KB per wave and stage
     extern __shared__ uint4 lds4[];
     __shared__ Blocks ring[128];
@@ -686,8 +700,9 @@ __global__ __launch_bounds__(64 * rows_waves(DT), DT <= 4 ? 2 : 1) void k_attend
     carry_init(cy);
     const int first = g.begin + split * g.per, count = min(g.tiles, (split + 1) * g.per) - split * g.per;
     // load u = wave + i * W of a stage: K of its blocks, then V, a kilobyte each
-    uint4 in[LOADS];
-    auto fetch = [&](int t, auto block_of) {  // the stage from tile t on
+    typedef uint4 Load[LOADS];
+    Load in0, in1;  // of even and odd stages
+    auto fetch = [&](Load& in, int t, auto block_of) {  // the stage from tile t on
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
             const int u = wave + i * W;
@@ -697,7 +712,7 @@ __global__ __launch_bounds__(64 * rows_waves(DT), DT <= 4 ? 2 : 1) void k_attend
             in[i] = ld16(a.c.codes + (int64_t)block * KB + (v % DT) * 1024 + lane * 16);
         }
     };
-    auto put = [&](int buf) {
+    auto put = [&](const Load& in, int buf) {
         uint8_t* to = lds + buf * BUF;
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
@@ -726,32 +741,24 @@ __global__ __launch_bounds__(64 * rows_waves(DT), DT <= 4 ? 2 : 1) void k_attend
         load_q<32, DT>(a, row, head, gl, w0 + col < r0 + nr, raw);
         if (EXT && a.alibi) slope = a.alibi[head];
         bl = find(0, page);
-        if (count > 0) fetch(0, [&](int t, int which) { return which ? lane_of(bl.v, t) : lane_of(bl.k, t); });
+        if (count > 0) fetch(in0, 0, [&](int t, int which) { return which ? lane_of(bl.v, t) : lane_of(bl.k, t); });
         halves<DT, ND>(raw, a.flip, qh, qs);
     }
     auto first_block = [&](int t, int which) { return which ? lane_of(bl.v, t) : lane_of(bl.k, t); };
     if (wave == 0) keep(0, bl);
-    if (count > 0) put(0);
-    if (STAGE < count) {
-        fetch(STAGE, first_block);
-        put(1);
-    }
-    if (2 * STAGE < count) fetch(2 * STAGE, first_block);
+    if (STAGE < count) fetch(in1, STAGE, first_block);
+    if (count > 0) put(in0, 0);
+    if (2 * STAGE < count) fetch(in0, 2 * STAGE, first_block);
     __syncthreads();
-    h8 k[2 * DT];
-    auto key = [&](const uint8_t* block) {
-#pragma unroll
-        for (int j = 0; j < 2 * DT; ++j) k[j] = reinterpret_cast<const h8*>(block)[j * 64 + lane];
+    auto scale_of = [&](int t, bool v) {
+        const Blocks& b = ring[t & 127];
+        return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v ? b.vs : b.ks)));
     };
-    constexpr bool EARLY = DT <= 6;      // (more dimensions: K at its block's beginning, the registers are needed)
-    constexpr int VH = EARLY ? 2 * DT : 6;  // pieces of V ahead of the exponentials
-    if (EARLY) key(lds);
-    int buf = 0;  // of the stage, and of the two behind it
-    for (int t = 0; t < count; t += STAGE) {
-        const int buf1 = buf == BUFS - 1 ? 0 : buf + 1, buf2 = buf1 == BUFS - 1 ? 0 : buf1 + 1;
-        if (t + 2 * STAGE < count) put(buf2);
-        if (t + 3 * STAGE < count) fetch(t + 3 * STAGE, ring_block);
-        if (wave == 0) {
+    constexpr int VH = DT < 4 ? 2 * DT : 8;  // pieces of V that are read ahead of the exponentials
+    auto stage = [&](int t, int buf, Load& in) {  // `in`: holds the next stage
+        if (t + STAGE < count) put(in, buf ^ 1);
+        if (t + 3 * STAGE < count) fetch(in, t + 3 * STAGE, ring_block);
+        if (wave == 0) {  // (the steps are one stage apart: each waits for what the one before asked for)
             const int from = (t & ~63) + 64, at = t & 63;
             if (from < count) {
                 if (at == 0) page = look(from);
@@ -761,17 +768,15 @@ __global__ __launch_bounds__(64 * rows_waves(DT), DT <= 4 ? 2 : 1) void k_attend
         }
 #pragma unroll
         for (int b = 0; b < STAGE; ++b) {
-            if (t + b >= count) break;
             const int t0 = (first + t + b) * KV_BLOCK;
-            const uint8_t* block = lds + buf * BUF + 2 * b * HB;
-            const uint8_t* next = b + 1 < STAGE ? block + 2 * HB : lds + buf1 * BUF;  // (behind the last block: what is there)
-            if (t0 >= some_hi || t0 + KV_BLOCK <= some_lo) {
-                if (EARLY) key(next);
-                continue;
-            }
-            if (!EARLY) key(block);
-            const float ks = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(ring[(t + b) & 127].ks)));
-            const float vs = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(ring[(t + b) & 127].vs)));
+            if (t + b >= count || t0 >= some_hi || t0 + KV_BLOCK <= some_lo) continue;
+            const h8* from = reinterpret_cast<const h8*>(lds + buf * BUF + 2 * b * HB) + lane;
+            const float ks = scale_of(t + b, false);
+            float vs = scale_of(t + b, true), c;
+            h8 k[2 * DT], v[2 * DT];
+#pragma unroll
+            for (int j = 0; j < 2 * DT; ++j) k[j] = from[j * 64];
+            __builtin_amdgcn_sched_barrier(0);
             v16f acc = {};
 #pragma unroll
             for (int j = 0; j < 2 * DT; ++j) {
@@ -781,18 +786,16 @@ __global__ __launch_bounds__(64 * rows_waves(DT), DT <= 4 ? 2 : 1) void k_attend
             float x[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) x[i] = acc[i];
-            h8 v[2 * DT];
-            const h8* value = reinterpret_cast<const h8*>(block + HB) + lane;
-            const auto w = weights<32, DT, ND, EXT>(cy, a, x, qs, slope, pos, ks, vs, t0, gl, lo, hi,
-                                                    t0 < whole_lo || t0 + KV_BLOCK > whole_hi, [&] {
+            follow(cy, see_scores<32, DT, EXT>(a, x, c, qs, slope, pos, ks, t0, gl, lo, hi, t0 < whole_lo || t0 + KV_BLOCK > whole_hi));
+            follow_value(cy, x, vs);
 #pragma unroll
-                                                        for (int i = 0; i < VH; ++i) v[i] = value[i * 64];
-                                                        if (EARLY) key(next);
-                                                        __builtin_amdgcn_sched_barrier(0);
-                                                    });
+            for (int i = 0; i < VH; ++i) v[i] = from[HB / 16 + i * 64];
+            __builtin_amdgcn_sched_barrier(0);
+            const auto w = weights<32, DT, ND>(cy, x, c, vs);
 #pragma unroll
             for (int i = 0; i < DT; ++i) {
-                if (2 * i + VH < 2 * DT) v[2 * i + VH] = value[(2 * i + VH) * 64], v[2 * i + VH + 1] = value[(2 * i + VH + 1) * 64];
+                if (2 * i + VH < 2 * DT)
+                    v[2 * i + VH] = from[HB / 16 + (2 * i + VH) * 64], v[2 * i + VH + 1] = from[HB / 16 + (2 * i + VH + 1) * 64];
                 cy.o[i] = value_mfma<32>(v[2 * i], w.p[0], cy.o[i]);
                 cy.o[i] = value_mfma<32>(v[2 * i + 1], w.p[1], cy.o[i]);
                 if constexpr (ND == 3) {
@@ -801,8 +804,11 @@ __global__ __launch_bounds__(64 * rows_waves(DT), DT <= 4 ? 2 : 1) void k_attend
                 }
             }
         }
-        buf = buf1;
         __syncthreads();
+    };
+    for (int t = 0; t < count; t += 2 * STAGE) {
+        stage(t, 0, in1);
+        if (t + STAGE < count) stage(t + STAGE, 1, in0);
     }
     cy.l = row_sum<32>(cy.l);
     if (w0 + col >= r0 + nr) return;
@@ -1124,8 +1130,8 @@ template <int DT>
 void launch_dt(const AttendArgs& a, hipStream_t st) {
     const bool ext = a.cap > 0.0f || a.alibi, wide = a.type == JX_TYPE_F32;
     if (a.tile_rows > 32)
-        launch_k(JX_ATTEND_FORM(k_attend_rows, DT), (unsigned)((int64_t)a.b.n_seqs * a.splits * a.row_tiles * a.c.H), 64 * rows_waves(DT),
-                 (size_t)BUFS * rows_stage(DT) * 4096 * DT, a, st);
+        launch_k(JX_ATTEND_FORM(k_attend_rows, DT), (unsigned)((int64_t)a.b.n_seqs * a.splits * a.row_tiles * a.c.H), 64 * ROWS_W,
+                 (size_t)2 * STAGE * 4096 * DT, a, st);
     else if (a.rows_cap <= 16)
         launch_form<16, DT>(a, ext, wide, st);
     else
@@ -1164,7 +1170,7 @@ AttendPlan attend_plan(const jx_kv_cache& c, const jx_kv_batch& b, const jx_atte
         p.partials = 2 * (int64_t)p.waves;
         return p;
     }
-    p.tile_rows = 32 * rows_waves(DT);
+    p.tile_rows = 32 * ROWS_W;
     p.row_tiles = (int)((rows + p.tile_rows - 1) / p.tile_rows);
     p.rows_cap = (int)std::min<int64_t>(p.tile_rows, rows);
     const int64_t items = (int64_t)b.n_seqs * p.row_tiles * c.n_kv_heads;
