@@ -901,7 +901,7 @@ __device__ __forceinline__ void join_row(const AttendArgs& a, int n, int rr, int
     }
 }
 
-// Rows that k_attend divided.  blockIdx.x as there without the splits, blockIdx.y = row of the row tile.
+// Rows that k_attend_rows divided: a wave for each row of a row tile, blockIdx.x as there without the splits
 __global__ __launch_bounds__(256) void k_attend_join(const AttendArgs a) {
     int item = blockIdx.x;
     const int kvh = item % a.c.H;
@@ -909,13 +909,16 @@ __global__ __launch_bounds__(256) void k_attend_join(const AttendArgs a) {
     const int rt = item % a.row_tiles, seq = item / a.row_tiles;
     const int failed = *a.c.status;
     const KvSeq s = kv_seq(a.c, a.b, seq);
-    const int rows = s.n * a.G, r = rt * a.tile_rows + blockIdx.y;
-    if (r >= rows) return;
-    const Range g = range_of(a, s, rt * a.tile_rows, min(a.tile_rows, rows - rt * a.tile_rows));
+    const int rows = s.n * a.G, r0 = rt * a.tile_rows;
+    if (r0 >= rows) return;
+    const int nr = min(a.tile_rows, rows - r0);
+    const Range g = range_of(a, s, r0, nr);
     if (g.n == 1) return;
-    const int64_t to = (int64_t)(s.row0 + r / a.G) * a.out_stride + (int64_t)(kvh * a.G + r % a.G) * a.c.D;
-    join_row<4>(a, g.n, blockIdx.y, to, failed,
-             [&](int i) { return (((int64_t)seq * a.splits + i) * a.row_tiles + rt) * a.c.H + kvh; });
+    for (int rr = blockIdx.y * 4 + (threadIdx.x >> 6); rr < nr; rr += gridDim.y * 4) {
+        const int r = r0 + rr;
+        const int64_t to = (int64_t)(s.row0 + r / a.G) * a.out_stride + (int64_t)(kvh * a.G + r % a.G) * a.c.D;
+        join_row<1>(a, g.n, rr, to, failed, [&](int i) { return (((int64_t)seq * a.splits + i) * a.row_tiles + rt) * a.c.H + kvh; });
+    }
 }
 
 // ---------------------------------------------------------------- few rows: the tiles of the whole batch in equal shares
@@ -1174,8 +1177,9 @@ AttendPlan attend_plan(const jx_kv_cache& c, const jx_kv_batch& b, const jx_atte
     p.row_tiles = (int)((rows + p.tile_rows - 1) / p.tile_rows);
     p.rows_cap = (int)std::min<int64_t>(p.tile_rows, rows);
     const int64_t items = (int64_t)b.n_seqs * p.row_tiles * c.n_kv_heads;
-    // a workgroup for each of the 256 CUs, of at least 16 tiles
-    const int64_t splits = std::max<int64_t>(1, std::min<int64_t>(256 / std::max<int64_t>(1, items), tiles / 16));
+    // Two workgroups share a CU, and sequences of several lengths need more to even out: up to 2048 of at least 16 tiles.  Five
+    // pieces of prompts (440 workgroups undivided): 113 us undivided, 70 in two parts, 50 in five, and the join
+    const int64_t splits = std::max<int64_t>(1, std::min<int64_t>(2048 / std::max<int64_t>(1, items), tiles / 16));
     p.chunk = (int)((tiles + splits - 1) / splits);
     p.splits = (int)((tiles + p.chunk - 1) / p.chunk);
     if (p.splits > 1) p.partials = items * p.splits;
@@ -1197,7 +1201,7 @@ void launch_attend(const AttendArgs& a, hipStream_t st) {
     if (a.waves)  // few sequences and heads: a workgroup per row (many partials each); many: one for all rows
         hipLaunchKernelGGL(k_attend_stream_join, dim3(pairs, pairs <= 128 ? a.rows_cap : 1), dim3(256), 0, st, a);
     else if (a.splits > 1)
-        hipLaunchKernelGGL(k_attend_join, dim3(pairs * a.row_tiles, a.rows_cap), dim3(256), 0, st, a);
+        hipLaunchKernelGGL(k_attend_join, dim3(pairs * a.row_tiles, (a.rows_cap + 31) / 32), dim3(256), 0, st, a);
 }
 
 }  // namespace jx
