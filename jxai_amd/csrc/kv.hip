@@ -40,7 +40,26 @@ struct AppendArgs {
     const void *k, *v;
     int64_t stride;
     int blocks;  // of a sequence's rows at most
+    bool vec;    // rows aligned to 16 bytes
 };
+
+// N consecutive values; vec: aligned to N of them (or to 16 bytes)
+template <typename T, int N>
+__device__ __forceinline__ void load_values(const T* p, bool vec, float* v) {
+    if (vec) {
+        typedef T V __attribute__((ext_vector_type(N * sizeof(T) > 16 ? 16 / sizeof(T) : N)));
+        constexpr int M = sizeof(V) / sizeof(T);
+#pragma unroll
+        for (int i = 0; i < N; i += M) {
+            const V u = *reinterpret_cast<const V*>(p + i);
+#pragma unroll
+            for (int k = 0; k < M; ++k) v[i + k] = widen<T>(u[k]);
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k) v[k] = widen<T>(p[k]);
+    }
+}
 
 // The block's scale after the new tokens (top: bits of their largest magnitude) and, if it grew, `grew`.
 __device__ __forceinline__ float new_scale(uint32_t top, float before, bool& grew) {
@@ -72,7 +91,9 @@ __device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
     return v;
 }
 
-// One wave for one block of 32 tokens of a kv head, K (blockIdx.z = 0) or V.
+// One wave for one block of 32 tokens of a kv head, K (blockIdx.z = 0) or V.  Bound by HBM for prompts (each lane's loads and
+// stores are 8 to 64 bytes in a row: 33.5 MB in and 16.8 out take 17 us), by the chain status, length, page, value, code
+// for single tokens, whose codes are written byte by byte without reading the block.
 template <typename T, int DT>
 __global__ __launch_bounds__(64) void k_append(const AppendArgs a) {
     if (*a.c.status) return;
@@ -102,18 +123,81 @@ __global__ __launch_bounds__(64) void k_append(const AppendArgs a) {
     const T* x = reinterpret_cast<const T*>(which ? a.v : a.k) + (int64_t)head * a.c.D + (int64_t)(s.row0 - begin) * a.stride;
     bool grew;
     uint32_t top = 0;
+    auto code = [&](float v, float now, float inv, float half) { return (uint32_t)((inv > 0.0f ? nearest(v, now, inv, half) : 0) & 255); };
+    const int lo = max(begin, t0), hi = min(s.len, t0 + KV_BLOCK);  // the new tokens
+    // the block's earlier codes at a scale that grew: K's rows below lo, V's bytes
+    auto recode_k = [&](float now) {
+        uint4* at = reinterpret_cast<uint4*>(codes) + h * 32 + r;
+        if (t0 + r < lo)
+#pragma unroll
+            for (int j = 0; j < DT; ++j) {
+                const uint4 u = at[j * 64];
+                at[j * 64] = make_uint4(recode4(u.x, before, now), recode4(u.y, before, now), recode4(u.z, before, now), recode4(u.w, before, now));
+            }
+    };
+    auto token_of = [&](int k) { return t0 + 8 * (2 * ((k >> 2) & 1) + (k >> 3)) + 4 * h + (k & 3); };  // of byte k of the lane half's pieces
+    if (hi - lo == 1) {
+        // one new token: the lane's values lane + 64 i
+        constexpr int N = (DT + 1) / 2;
+        float v[N];
+        const T* row = x + (int64_t)lo * a.stride;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            v[i] = lane + 64 * i < 32 * DT ? widen<T>(row[lane + 64 * i]) : 0.0f;
+            top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+        }
+        const float now = new_scale(wave_umax(top), before, grew);
+        const float inv = now > 0.0f ? 1.0f / now : 0.0f, half = 0.5f * now;
+        if (lane == 0) a.c.scales[index] = now;
+        if (grew && lo > t0) {
+            if (which == 0) {
+                recode_k(now);
+            } else {
+                uint4* at = reinterpret_cast<uint4*>(codes) + h * 32 * DT + r;
+                uint32_t keep[4] = {};
+#pragma unroll
+                for (int k = 0; k < 16; ++k)
+                    if (token_of(k) < lo) keep[k >> 2] |= 255u << (8 * (k & 3));
+#pragma unroll
+                for (int j = 0; j < DT; ++j) {
+                    const uint4 u = at[j * 32];
+                    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+                    uint32_t o[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) o[k] = keep[k] ? (recode4(w[k], before, now) & keep[k]) | (w[k] & ~keep[k]) : w[k];
+                    at[j * 32] = make_uint4(o[0], o[1], o[2], o[3]);
+                }
+            }
+            // the new token's bytes lie in words that other lanes have just stored whole
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+        const int t = lo - t0, ta = t >> 3, th = (t >> 2) & 1;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int d = lane + 64 * i;
+            if (d >= 32 * DT) break;
+            const int at = which == 0 ? (d >> 4) * 512 + t * 16 + (d & 15) : (th * 32 * DT + d) * 16 + 8 * (ta & 1) + 4 * (ta >> 1) + (t & 3);
+            codes[at] = (int8_t)code(v[i], now, inv, half);
+        }
+        return;
+    }
     if (which == 0) {
         // lane (h, r): dimensions 32 j + 16 h .. + 15 of token r
-        const int t = t0 + r;
-        const bool fresh = t >= begin && t < s.len;
+        const bool fresh = t0 + r >= lo && t0 + r < hi;
         float v[DT][16];
+#pragma unroll
+        for (int j = 0; j < DT; ++j) {
+            if (fresh) {
+                load_values<T, 16>(x + (int64_t)(t0 + r) * a.stride + 32 * j + 16 * h, a.vec, v[j]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 16; ++k) v[j][k] = 0.0f;
+            }
+        }
 #pragma unroll
         for (int j = 0; j < DT; ++j)
 #pragma unroll
-            for (int k = 0; k < 16; ++k) {
-                v[j][k] = fresh ? widen<T>(x[(int64_t)t * a.stride + 32 * j + 16 * h + k]) : 0.0f;
-                top = max(top, __float_as_uint(v[j][k]) & 0x7FFFFFFFu);
-            }
+            for (int k = 0; k < 16; ++k) top = max(top, __float_as_uint(v[j][k]) & 0x7FFFFFFFu);
         const float now = new_scale(wave_umax(top), before, grew);
         const float inv = now > 0.0f ? 1.0f / now : 0.0f, half = 0.5f * now;
         if (lane == 0) a.c.scales[index] = now;
@@ -123,55 +207,60 @@ __global__ __launch_bounds__(64) void k_append(const AppendArgs a) {
             for (int j = 0; j < DT; ++j) {
                 uint32_t w[4] = {};
 #pragma unroll
-                for (int k = 0; k < 16; ++k)
-                    w[k >> 2] |= (uint32_t)((inv > 0.0f ? nearest(v[j][k], now, inv, half) : 0) & 255) << (8 * (k & 3));
+                for (int k = 0; k < 16; ++k) w[k >> 2] |= code(v[j][k], now, inv, half) << (8 * (k & 3));
                 to[j * 64] = make_uint4(w[0], w[1], w[2], w[3]);
             }
-        } else if (grew && t < begin) {
-#pragma unroll
-            for (int j = 0; j < DT; ++j) {
-                const uint4 u = to[j * 64];
-                to[j * 64] = make_uint4(recode4(u.x, before, now), recode4(u.y, before, now), recode4(u.z, before, now),
-                                        recode4(u.w, before, now));
-            }
+        } else if (grew) {
+            recode_k(now);
         }
     } else {
-        // lane (h, r): dimensions 32 j + r of the 16 tokens 8 a + 4 h + b
-        float v[DT][16];
+        // lane (h, r): dimensions 128 j + 4 r .. + 3 of the 16 tokens 8 a + 4 h + b, four pieces of 16 bytes in a row
+        constexpr int N = (DT + 3) / 4;
+        float v[N][16][4];
 #pragma unroll
-        for (int k = 0; k < 16; ++k) {
-            const int t = t0 + 8 * (2 * ((k >> 2) & 1) + (k >> 3)) + 4 * h + (k & 3);  // byte k
-            const bool fresh = t >= begin && t < s.len;
+        for (int j = 0; j < N; ++j) {
+            const int d = 128 * j + 4 * r;
 #pragma unroll
-            for (int j = 0; j < DT; ++j) {
-                v[j][k] = fresh ? widen<T>(x[(int64_t)t * a.stride + 32 * j + r]) : 0.0f;
-                top = max(top, __float_as_uint(v[j][k]) & 0x7FFFFFFFu);
+            for (int k = 0; k < 16; ++k) {
+                const int t = token_of(k);
+                if (d < 32 * DT && t >= lo && t < hi) {
+                    load_values<T, 4>(x + (int64_t)t * a.stride + d, a.vec, v[j][k]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[j][k][i] = 0.0f;
+                }
             }
         }
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+#pragma unroll
+            for (int k = 0; k < 16; ++k)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(v[j][k][i]) & 0x7FFFFFFFu);
         const float now = new_scale(wave_umax(top), before, grew);
         const float inv = now > 0.0f ? 1.0f / now : 0.0f, half = 0.5f * now;
         if (lane == 0) a.c.scales[index] = now;
-        uint32_t keep[4] = {};  // bytes of earlier tokens, of new tokens
-        uint32_t put[4] = {};
+        uint32_t keep[4] = {}, put[4] = {};  // bytes of earlier tokens, of new tokens
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
-            const int t = t0 + 8 * (2 * ((k >> 2) & 1) + (k >> 3)) + 4 * h + (k & 3);
-            const uint32_t m = 255u << (8 * (k & 3));
-            if (t < begin) keep[k >> 2] |= m;
-            if (t >= begin && t < s.len) put[k >> 2] |= m;
+            const int t = token_of(k);
+            if (t < lo) keep[k >> 2] |= 255u << (8 * (k & 3));
+            if (t >= lo && t < hi) put[k >> 2] |= 255u << (8 * (k & 3));
         }
         const bool whole = (put[0] & put[1] & put[2] & put[3]) == 0xFFFFFFFFu;
         const bool some = (put[0] | put[1] | put[2] | put[3]) != 0 || grew;
-        uint4* to = reinterpret_cast<uint4*>(codes) + h * a.c.D + r;
-        if (some) {
 #pragma unroll
-            for (int j = 0; j < DT; ++j) {
+        for (int j = 0; j < N; ++j) {
+            const int d = 128 * j + 4 * r;
+            if (d >= 32 * DT || !some) continue;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint4* to = reinterpret_cast<uint4*>(codes) + h * 32 * DT + d + i;
                 uint32_t w[4] = {};
 #pragma unroll
-                for (int k = 0; k < 16; ++k)
-                    w[k >> 2] |= (uint32_t)((inv > 0.0f ? nearest(v[j][k], now, inv, half) : 0) & 255) << (8 * (k & 3));
+                for (int k = 0; k < 16; ++k) w[k >> 2] |= code(v[j][k][i], now, inv, half) << (8 * (k & 3));
                 if (!whole) {
-                    const uint4 u4 = to[j * 32];
+                    const uint4 u4 = *to;
                     const uint32_t u[4] = {u4.x, u4.y, u4.z, u4.w};
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
@@ -179,7 +268,7 @@ __global__ __launch_bounds__(64) void k_append(const AppendArgs a) {
                         w[k] = (w[k] & put[k]) | (old & keep[k]) | (u[k] & ~(put[k] | keep[k]));
                     }
                 }
-                to[j * 32] = make_uint4(w[0], w[1], w[2], w[3]);
+                *to = make_uint4(w[0], w[1], w[2], w[3]);
             }
         }
     }
@@ -267,8 +356,9 @@ __device__ __forceinline__ int any(int v, int* lds) {  // workgroup-wide or
 // One workgroup: global memory written before a barrier is read after it through the L2
 __device__ __forceinline__ int peek(const int32_t* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 __device__ __forceinline__ void poke(int32_t* p, int v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+// (its stores and atomics have reached the L2 once they are counted as done; peek reads there)
 __device__ __forceinline__ void settle() {
-    __threadfence();
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
 }
 
@@ -519,7 +609,9 @@ __global__ __launch_bounds__(PLAN) void k_compact(const PageArgs a) {
     }
 }
 
-// The copies that the bookkeeping listed, in every layer, and a compaction's new page numbers in the tables.
+// The copies that the bookkeeping listed, in every layer, and a compaction's new page numbers in the tables.  16 KB per workgroup
+// and turn, all of it in flight: bound by HBM (957 MB read and written in 176 us, 5.4 TB/s, where a plain copy of 1 GiB
+// reaches 5.24; 185 us without the non-temporal hints).
 __global__ __launch_bounds__(256) void k_copy(const PageArgs a) {
     const KvView& c = a.c;
     const Book b = book_of(a.scratch, c);
@@ -539,10 +631,10 @@ __global__ __launch_bounds__(256) void k_copy(const PageArgs a) {
         uint4 v[SEG / 4096];
 #pragma unroll
         for (int k = 0; k < SEG / 4096; ++k)
-            if (k * 4096 + threadIdx.x * 16 < n) v[k] = ld16(s + k * 4096 + threadIdx.x * 16);
+            if (k * 4096 + threadIdx.x * 16 < n) v[k] = ld_stream16(s + k * 4096 + threadIdx.x * 16);
 #pragma unroll
         for (int k = 0; k < SEG / 4096; ++k)
-            if (k * 4096 + threadIdx.x * 16 < n) *reinterpret_cast<uint4*>(d + k * 4096 + threadIdx.x * 16) = v[k];
+            if (k * 4096 + threadIdx.x * 16 < n) __builtin_nontemporal_store(u32x4{v[k].x, v[k].y, v[k].z, v[k].w}, reinterpret_cast<u32x4*>(d + k * 4096 + threadIdx.x * 16));
         if (seg == 0) {
             float* sc = c.scales + layer * a.layer_scales;
             for (int k = threadIdx.x; k < page_scales; k += 256) sc[(int64_t)to * page_scales + k] = sc[(int64_t)from * page_scales + k];
@@ -750,6 +842,7 @@ int jx_kv_append(const jx_kv_cache* c, const jx_kv_batch* b, int32_t layer, int3
     a.k = k;
     a.v = v;
     a.stride = row_stride ? row_stride : width;
+    a.vec = aligned(k, 16) && aligned(v, 16) && a.stride * size % 16 == 0;
     const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     if (type == JX_TYPE_F32)
         append_type<float>(a, st);
