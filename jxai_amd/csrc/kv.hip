@@ -23,14 +23,14 @@ __device__ __forceinline__ float widen<_Float16>(_Float16 v) { return (float)v; 
 template <>
 __device__ __forceinline__ float widen<__bf16>(__bf16 v) { return (float)v; }
 
-// The integer nearest to v / s (ties to the even one), |v / s| at most 127 and a rounding: inv = 1 / s, half = s / 2.  The
+// The integer nearest to v / s (ties to the even one), |v| at most 127 s and a rounding: inv = 1 / s, half = s / 2.  The
 // product's rounding can miss by one next to the middle of two integers, so the remainder decides: v - q s is a
 // multiple of half an ulp of s and below 2 s, hence exact from one fused multiply-add where it is near s / 2.
 __device__ __forceinline__ int nearest(float v, float s, float inv, float half) {
     float q = __builtin_rintf(v * inv);
     const float e = __builtin_fmaf(-q, s, v), ae = __builtin_fabsf(e);
     if (ae > half || (ae == half && ((int)q & 1))) q += __builtin_copysignf(1.0f, e);
-    return (int)fminf(fmaxf(q, -127.0f), 127.0f);
+    return (int)q;
 }
 
 struct AppendArgs {
@@ -74,14 +74,19 @@ __device__ __forceinline__ float new_scale(uint32_t top, float before, bool& gre
     return grew ? s : before;
 }
 
-// An earlier code at its block's new scale
-__device__ __forceinline__ int recode(int code, float before, float now) {
-    return (int)__builtin_rint((double)code * (double)before / (double)now);
+// An earlier code at its block's new scale: the integer nearest to code * before / now.  Both products have 31 bits, so their
+// difference in 64 bits is exact.
+__device__ __forceinline__ int recode(int code, float before, float now, float ratio) {
+    float q = __builtin_rintf((float)code * ratio);
+    const double e = (double)code * (double)before - (double)q * (double)now, ae = __builtin_fabs(e), half = 0.5 * (double)now;
+    if (ae > half || (ae == half && ((int)q & 1))) q += __builtin_copysignf(1.0f, (float)e);
+    return (int)q;
 }
 __device__ __forceinline__ uint32_t recode4(uint32_t w, float before, float now) {
+    const float ratio = before / now;
     uint32_t r = 0;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) r |= (uint32_t)(recode((int)(int8_t)(w >> (8 * k)), before, now) & 255) << (8 * k);
+    for (int k = 0; k < 4; ++k) r |= (uint32_t)(recode((int)(int8_t)(w >> (8 * k)), before, now, ratio) & 255) << (8 * k);
     return r;
 }
 
@@ -92,7 +97,7 @@ __device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
 }
 
 // One wave for one block of 32 tokens of a kv head, K (blockIdx.z = 0) or V.  Bound by HBM for prompts (each lane's loads and
-// stores are 8 to 64 bytes in a row: 33.5 MB in and 16.8 out take 17 us), by the chain status, length, page, value, code
+// stores are 8 to 64 bytes in a row: 33.5 MB in and 16.8 out take 20 us), by the chain status, length, page, value, code
 // for single tokens, whose codes are written byte by byte without reading the block.
 template <typename T, int DT>
 __global__ __launch_bounds__(64) void k_append(const AppendArgs a) {
@@ -185,15 +190,10 @@ __global__ __launch_bounds__(64) void k_append(const AppendArgs a) {
         // lane (h, r): dimensions 32 j + 16 h .. + 15 of token r
         const bool fresh = t0 + r >= lo && t0 + r < hi;
         float v[DT][16];
+        // (lanes without a new token read the nearest one, which changes no maximum: all loads are in flight together)
+        const T* row = x + (int64_t)min(max(t0 + r, lo), hi - 1) * a.stride + 16 * h;
 #pragma unroll
-        for (int j = 0; j < DT; ++j) {
-            if (fresh) {
-                load_values<T, 16>(x + (int64_t)(t0 + r) * a.stride + 32 * j + 16 * h, a.vec, v[j]);
-            } else {
-#pragma unroll
-                for (int k = 0; k < 16; ++k) v[j][k] = 0.0f;
-            }
-        }
+        for (int j = 0; j < DT; ++j) load_values<T, 16>(row + 32 * j, a.vec, v[j]);
 #pragma unroll
         for (int j = 0; j < DT; ++j)
 #pragma unroll
@@ -219,17 +219,10 @@ __global__ __launch_bounds__(64) void k_append(const AppendArgs a) {
         float v[N][16][4];
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            const int d = 128 * j + 4 * r;
+            const int d = 128 * j + 4 * r < 32 * DT ? 128 * j + 4 * r : 4 * r;
 #pragma unroll
-            for (int k = 0; k < 16; ++k) {
-                const int t = token_of(k);
-                if (d < 32 * DT && t >= lo && t < hi) {
-                    load_values<T, 4>(x + (int64_t)t * a.stride + d, a.vec, v[j][k]);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) v[j][k][i] = 0.0f;
-                }
-            }
+            for (int k = 0; k < 16; ++k)
+                load_values<T, 4>(x + (int64_t)min(max(token_of(k), lo), hi - 1) * a.stride + (d < 32 * DT ? d : 0), a.vec, v[j][k]);
         }
 #pragma unroll
         for (int j = 0; j < N; ++j)
