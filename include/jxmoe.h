@@ -240,12 +240,11 @@ int jx_quantize_row_q8_0(const float* x, void* blocks, int64_t k);
  *   ref    int32 [n_pages]: how many slots hold a page (0: free)
  *   status int32 [JX_KV_STATUS_WORDS]: word 0 the JX_KV_* bits below, word 1 the pages in use after jx_kv_compact
  *   scratch int32 [jx_kv_scratch_words()]: workspace of the page operations
- * The first JX_KV_* bit that a call of jx_kv_append sets may leave its other sequences' tokens written.
  * A program zeroes len, ref and status once; codes, scales, table and scratch need no initial values.
  *
  * Errors that only the device can see set a bit of the status word.  While it is not zero, jx_kv_append and the page
  * operations do nothing and jx_kv_attention writes NaN: read it (4 bytes) where results are read, zero it to go on.
- * A page operation that reports changed nothing.
+ * A page operation that reports changed nothing; an append that reports may have written its other sequences' tokens.
  *
  * Every call is enqueued on `stream` (NULL = default stream), returns without synchronizing, allocates nothing, reads
  * lengths, tables and lists on the device only and may be captured in a graph.  Calls that change a cache must be
@@ -320,8 +319,8 @@ int jx_kv_append(const jx_kv_cache* cache, const jx_kv_batch* batch, int32_t lay
  *   out = sum_t exp(x_t) V_t / sum_t exp(x_t), zeros where nothing is visible
  * visible: causal: t <= p, otherwise every token of the sequence; window > 0: also t > p - window.
  * q, out: [n_rows][n_heads][head_dim] of `type` with q_stride / out_stride elements between rows (0: n_heads * head_dim),
- * any alignment of the type; out may be q.  type F32 keeps 21 bits of q against its row's largest value and the
- * weights in 22 bits; F16 and BF16 keep 14 and 11.  A row of q with a value that is not finite gives NaN; one whose
+ * any alignment of the type; out may be q.  type F32 keeps at least 21 bits of q against its row's largest value
+ * and 22 of the weights; F16 and BF16 keep 14 and 11.  A row of q with a value that is not finite gives NaN; one whose
  * values are all below 2^-100 counts as zeros.
  * ws: device memory of jx_kv_attention_workspace() bytes (0: may be NULL), 16-byte aligned, for this call alone. */
 typedef struct jx_attention {

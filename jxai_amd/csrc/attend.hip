@@ -4,6 +4,7 @@
 // tokens at a time, everything in registers:
 //   S^T = K Q^T   32x32x32 int8 MFMAs: the codes of K as they lie in memory (one 16-byte load per lane and 32 dimensions)
 //                 against q as two (fp32: three) signed digits of 7 bits, exact in int32
+//                 (many rows: fp16 MFMAs on K converted once for the workgroup)
 //   x = S * (scale of the row * scale of K's block * softmax scale), in units of log2; one scale per tile and lane
 //   p = exp2(x - m), m a reference maximum of the row, at most 2^6 behind the true one
 //   O^T += V^T P^T   32x32x16 fp16 MFMAs.  V's codes lie so that a lane's 16 bytes are the 16 tokens whose weights the same
